@@ -87,6 +87,14 @@ void paged_kv_append(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor k_p
 void paged_attention_decode(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor block_tables,
                             torch::Tensor seq_lens, torch::Tensor out, torch::Tensor part_o, torch::Tensor part_ml,
                             int64_t tokens_per_split, double scale);
+torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
+                                     torch::Tensor lens, torch::Tensor pages, int64_t L,
+                                     c10::optional<torch::Tensor> qlens, double scale);
+void page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor dst,
+               c10::optional<torch::Tensor> counts);
+std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10::optional<torch::Tensor> draft,
+                                                      torch::Tensor tokens, torch::Tensor uniforms,
+                                                      c10::optional<torch::Tensor> lens, double threshold);
 void flash_attn_fwd_pp(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
                        bool causal, double scale, bool poly, c10::optional<torch::Tensor> trace, bool x2,
                        c10::optional<torch::Tensor> blk_ptr, c10::optional<torch::Tensor> blk_idx,
@@ -157,6 +165,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ep_grad_w", &scirs::ep_grad_w, "routing-weight gradient against peers' expert outputs");
   m.def("paged_kv_append", &scirs::paged_kv_append);
   m.def("paged_attention_decode", &scirs::paged_attention_decode);
+  m.def("paged_prefix_attention", &scirs::paged_prefix_attention,
+        "attention over the paged cache for a batch that shares a prefix");
+  m.def("page_copy", &scirs::page_copy, "copy pages of every layer's pools");
+  m.def("draft_verify", &scirs::draft_verify, "keep or replace drafted tokens");
   m.def("flash_attn_fwd_pp", &scirs::flash_attn_fwd_pp, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
         py::arg("lse"), py::arg("causal"), py::arg("scale"), py::arg("poly") = false,
         py::arg("trace") = py::none(), py::arg("x2") = false, py::arg("blk_ptr") = py::none(),

@@ -15,10 +15,13 @@
 
 #include "common.cuh"
 
+// Numbers go into messages through std::to_string: an extension that carries its own copy of libstdc++
+// (a toolchain without the shared one) crashes in operator<< of a number when torch has loaded another.
 #define SCIRS_CHECK_CUDA(expr)                                                                       \
   do {                                                                                               \
     cudaError_t _e = (expr);                                                                         \
-    TORCH_CHECK(_e == cudaSuccess, "CUDA error ", cudaGetErrorString(_e), " at ", __FILE__, ":", __LINE__); \
+    TORCH_CHECK(_e == cudaSuccess, "CUDA error ", cudaGetErrorString(_e), " at " __FILE__ ":",        \
+                std::to_string(__LINE__));                                                           \
   } while (0)
 
 #define SCIRS_CHECK_LAUNCH() SCIRS_CHECK_CUDA(cudaGetLastError())
@@ -41,6 +44,8 @@ int num_sms(int device);
 CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t inner, uint64_t outer,
                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                          CUtensorMapSwizzle swizzle);
+
+inline std::string num(int64_t v) { return std::to_string(v); }
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 

@@ -7,7 +7,9 @@ LayerNorm -> QKV GEMM -> append K/V (paged_kv_append) -> paged decode
 attention over the sequence's page chain -> projection GEMM (+residual) ->
 LayerNorm -> GELU MLP GEMMs -> final LayerNorm -> LM head -> next token.
 All layers share one page table (the pages of layer l live in layer l's
-pool at the same page ids).
+pool at the same page ids). Sequences can be forked (several samples of one
+prompt share its pages, and a step reads them once), and `verify` feeds a few
+drafted tokens per sequence at once and keeps those that the model confirms.
 
 Reference parity: the reference generates with its (placeholder) GPT on the
 CPU without a cache (scirs2-neural/src/models/architectures/gpt.rs); the
@@ -19,8 +21,9 @@ import torch
 
 from .. import _ext
 from ..ops import kernels as K
-from .kv_cache import BlockManager, BlockManagerConfig, KvPageConfig, KvPagePool
+from .kv_cache import BlockManager, BlockManagerConfig, InferenceError, KvPageConfig, KvPagePool
 from .paged_attention import PagedAttentionConfig, PagedAttentionForward
+from .speculative import verify_drafts
 
 
 class GPTGenerator:
@@ -35,7 +38,7 @@ class GPTGenerator:
         num_pages = num_pages or max_sequences * pages_per_seq
         pc = KvPageConfig(block_size=block_size, num_heads=self.H, head_dim=self.hd)
         self.pools = [KvPagePool(num_pages, pc, model.device) for _ in range(self.L)]
-        self.manager = BlockManager(self.pools[0], BlockManagerConfig(max_sequences, pages_per_seq))
+        self.manager = BlockManager(self.pools[0], BlockManagerConfig(max_sequences, pages_per_seq), self.pools)
         self.attn = PagedAttentionForward(PagedAttentionConfig(self.H, self.hd))
         self.max_len = max_len
         self._next_id = 0
@@ -79,18 +82,22 @@ class GPTGenerator:
         self.last_token[sid] = nxt
         return sid
 
-    @torch.no_grad()
-    def step(self, seq_ids: list[int], temperature: float = 0.0, generator=None) -> list[int]:
-        """Feed each sequence's pending token, return the next tokens."""
+    def fork(self, seq_id: int) -> int:
+        """A copy of a sequence (its tokens and its pending one) that goes its own way from here. The
+        two share their pages until one of them writes into one; step reads what a batch shares once."""
+        sid = self._next_id
+        self.manager.fork_sequence(seq_id, sid)
+        self._next_id += 1
+        self.last_token[sid] = self.last_token[seq_id]
+        return sid
+
+    def _decode(self, toks, posn, rows, pos, attend) -> torch.Tensor:
+        """Logits (fp32) of new tokens toks [n] at positions posn, whose keys and values go to the
+        (row, position) pairs; attend(q [n, H, hd], pool) is the attention over the cache."""
         m, fp, cfg = self.m, self.m.fp, self.cfg
         H, hd, D = self.H, self.hd, self.D
-        n = len(seq_ids)
+        n = toks.numel()
         dev = m.device
-        toks = torch.tensor([self.last_token[s] for s in seq_ids], dtype=torch.long, device=dev)
-        lens = [self.manager.seq_len(s) for s in seq_ids]
-        posn = torch.tensor(lens, dtype=torch.long, device=dev)
-        rows, pos = self.manager.reserve(seq_ids, [1] * n)
-        self.manager.sync()
         bf, f32 = torch.bfloat16, torch.float32
         x = (fp.w("wte")[toks].float() + fp.w("wpe")[posn].float()).to(bf).contiguous()
         ln = torch.empty(n, D, dtype=bf, device=dev)
@@ -99,9 +106,6 @@ class GPTGenerator:
         xm = torch.empty(n, D, dtype=bf, device=dev)
         h = torch.empty(n, cfg.intermediate_size, dtype=bf, device=dev)
         g = torch.empty(n, cfg.intermediate_size, dtype=bf, device=dev)
-        idx = torch.tensor([self.manager.row_of(s) for s in seq_ids], dtype=torch.long, device=dev)
-        bt = self.manager.block_tables[idx].contiguous()
-        sl = self.manager.seq_lens[idx].contiguous()
         eps = cfg.layer_norm_eps
         for l in range(self.L):
             p = f"h{l}."
@@ -109,8 +113,8 @@ class GPTGenerator:
             K.gemm(ln, fp.w(p + "attn.c_attn.weight"), qkv, bias=fp.w(p + "attn.c_attn.bias"))
             q3 = qkv.view(n, 3, H, hd)
             self._append(l, rows, pos, q3[:, 1], q3[:, 2])
-            att = self.attn.forward_batch(q3[:, 0].contiguous(), self.pools[l], bt, sl)
-            K.gemm(att.view(n, D), fp.w(p + "attn.c_proj.weight"), xm, epi=K.EPI_RESID,
+            att = attend(q3[:, 0], self.pools[l])
+            K.gemm(att.reshape(n, D), fp.w(p + "attn.c_proj.weight"), xm, epi=K.EPI_RESID,
                    bias=fp.w(p + "attn.c_proj.bias"), aux=x)
             K.layernorm_fwd(xm, fp.w(p + "ln_2.weight"), fp.w(p + "ln_2.bias"), ln, mu, rs, eps)
             K.gemm(ln, fp.w(p + "mlp.c_fc.weight"), g, epi=K.EPI_BIAS_GELU, bias=fp.w(p + "mlp.c_fc.bias"), out2=h)
@@ -120,7 +124,34 @@ class GPTGenerator:
         K.layernorm_fwd(x, fp.w("ln_f.weight"), fp.w("ln_f.bias"), ln, mu, rs, eps)
         logits = torch.empty(n, cfg.vocab_padded, dtype=bf, device=dev)
         K.gemm(ln, fp.w("wte"), logits)
-        lg = logits[:, : cfg.vocab_size].float()
+        return logits[:, : cfg.vocab_size].float()
+
+    def _cache_of(self, seq_ids: list[int]):
+        """Tables and lengths of the batch, and the pages that all its chains begin with."""
+        dev = self.m.device
+        idx = torch.tensor([self.manager.row_of(s) for s in seq_ids], dtype=torch.long, device=dev)
+        pages, shared = self.manager.shared_prefix(seq_ids) if len(seq_ids) > 1 else ([], 0)
+        return (self.manager.block_tables[idx].contiguous(), self.manager.seq_lens[idx].contiguous(),
+                torch.tensor(pages, dtype=torch.int32, device=dev), shared)
+
+    @torch.no_grad()
+    def step(self, seq_ids: list[int], temperature: float = 0.0, generator=None) -> list[int]:
+        """Feed each sequence's pending token, return the next tokens."""
+        n = len(seq_ids)
+        dev = self.m.device
+        toks = torch.tensor([self.last_token[s] for s in seq_ids], dtype=torch.long, device=dev)
+        lens = [self.manager.seq_len(s) for s in seq_ids]
+        posn = torch.tensor(lens, dtype=torch.long, device=dev)
+        rows, pos = self.manager.reserve(seq_ids, [1] * n)
+        self.manager.sync()
+        bt, sl, pages, shared = self._cache_of(seq_ids)
+
+        def attend(q, pool):
+            if shared:  # forked sequences: the pages they all begin with are read once
+                return self.attn.forward_shared_prefix(q, pool, bt, sl, pages, shared)
+            return self.attn.forward_batch(q.contiguous(), pool, bt, sl)
+
+        lg = self._decode(toks, posn, rows, pos, attend)
         if temperature > 0:
             nxt = torch.multinomial(torch.softmax(lg / temperature, -1), 1, generator=generator).view(-1)
         else:
@@ -130,9 +161,80 @@ class GPTGenerator:
             self.last_token[s] = t
         return out
 
-    def generate(self, prompts: list[torch.Tensor], max_new_tokens: int, temperature: float = 0.0) -> list[list[int]]:
-        """Greedy (temperature 0) or sampled continuation of every prompt."""
-        ids = [self.add_sequence(p) for p in prompts]
+    @torch.no_grad()
+    def verify(self, seq_ids: list[int], drafts: list[list[int]], draft_probs: torch.Tensor | None = None,
+               temperature: float = 0.0, uniforms: torch.Tensor | None = None, generator=None) -> list[list[int]]:
+        """One step of speculative decoding: feed each sequence's pending token and its drafted ones
+        (drafts[i], any number of them), keep the drafts that the model confirms, and return per
+        sequence those and the token that follows, which becomes its pending one.
+
+        draft_probs fp32 [B, n, vocab], n the largest number of drafts, holds the distributions that
+        the drafts were drawn from (None: the draft is certain of them); uniforms fp32 [B, n + 1] the
+        random numbers (default: drawn here). Temperature 0 keeps the drafts that equal the model's
+        own choice. The cache of rejected drafts is given back (speculative.verify_drafts)."""
+        B, dev, mgr = len(seq_ids), self.m.device, self.manager
+        if len(drafts) != B:
+            raise InferenceError("one list of drafts per sequence")
+        if len(set(seq_ids)) < B:
+            raise InferenceError("a sequence is verified once at a time")
+        counts = [1 + len(d) for d in drafts]
+        Q = max(counts)
+        lens = [mgr.seq_len(s) for s in seq_ids]
+        if any(a + c > self.cfg.max_position_embeddings for a, c in zip(lens, counts)):
+            raise InferenceError("sequence exceeds the model's positions")
+        fed = [t for s, d in zip(seq_ids, drafts) for t in (self.last_token[s], *d)]
+        if any(not 0 <= t < self.cfg.vocab_size for t in fed):
+            raise InferenceError("drafted token outside the vocabulary")
+        if draft_probs is not None and draft_probs.shape != (B, Q - 1, self.cfg.vocab_size):
+            raise InferenceError(f"draft_probs must be [{B}, {Q - 1}, {self.cfg.vocab_size}]")
+        if uniforms is not None and uniforms.shape != (B, Q):
+            raise InferenceError(f"uniforms must be [{B}, {Q}]")
+        toks = torch.tensor(fed, dtype=torch.long, device=dev)
+        posn = torch.tensor([a + i for a, c in zip(lens, counts) for i in range(c)], dtype=torch.long, device=dev)
+        at = torch.tensor([b * Q + i for b, c in enumerate(counts) for i in range(c)], dtype=torch.long, device=dev)
+        rows, pos = mgr.reserve(seq_ids, counts)
+        mgr.sync()
+        bt, sl, pages, shared = self._cache_of(seq_ids)
+        ql = torch.tensor(counts, dtype=torch.int32, device=dev)
+
+        def attend(q, pool):
+            q4 = torch.zeros(B * Q, self.H, self.hd, dtype=q.dtype, device=dev)
+            q4[at] = q
+            o = self.attn.forward_shared_prefix(q4.view(B, Q, self.H, self.hd), pool, bt, sl, pages, shared, ql)
+            return o.view(B * Q, self.H, self.hd)[at]
+
+        lg = self._decode(toks, posn, rows, pos, attend)
+        if temperature > 0:
+            p = torch.softmax(lg / temperature, -1)
+        else:
+            p = torch.zeros_like(lg).scatter_(1, torch.argmax(lg, -1, keepdim=True), 1.0)
+        target = torch.zeros(B * Q, p.shape[1], device=dev)
+        target[at] = p
+        dt = torch.tensor([list(d) + [-1] * (Q - 1 - len(d)) for d in drafts], dtype=torch.long).view(B, Q - 1).to(dev)
+        if uniforms is None:
+            uniforms = torch.rand(B, Q, device=dev, generator=generator)
+        kept, new = verify_drafts(target.view(B, Q, -1), draft_probs, dt, uniforms,
+                                  torch.tensor([c - 1 for c in counts], dtype=torch.int32, device=dev))
+        out = [t[: k + 1] for k, t in zip(kept.tolist(), new.tolist())]
+        nothing = any(t[-1] < 0 for t in out)  # NaN logits: leave every sequence as it was
+        for s, a, t in zip(seq_ids, lens, out):
+            mgr.truncate_sequence(s, a if nothing else a + len(t))
+            if not nothing:
+                self.last_token[s] = t[-1]
+        if nothing:
+            raise InferenceError("the model's probabilities hold no token to draw")
+        return out
+
+    def generate(self, prompts: list[torch.Tensor], max_new_tokens: int, temperature: float = 0.0,
+                 num_samples: int = 1) -> list[list[int]]:
+        """Greedy (temperature 0) or sampled continuation of every prompt, num_samples of each (prompt
+        by prompt; the prompt is processed once and forked)."""
+        if num_samples < 1:
+            raise ValueError("num_samples must be at least 1")
+        ids = []
+        for p in prompts:
+            ids.append(self.add_sequence(p))
+            ids += [self.fork(ids[-1]) for _ in range(num_samples - 1)]
         outs = {s: [self.last_token[s]] for s in ids}
         for _ in range(max_new_tokens - 1):
             for s, t in zip(ids, self.step(ids, temperature)):

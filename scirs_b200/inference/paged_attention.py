@@ -7,6 +7,12 @@ this is the split-key decode kernel of scirs_b200/csrc/paged_attention.cu
 (bandwidth-bound: each cached K/V byte is read once per sequence and KV head)
 followed by a combine kernel; on the CPU a PyTorch restatement.
 
+:meth:`PagedAttentionForward.forward_shared_prefix` is the same for a batch
+whose sequences begin with the same tokens (forks of one prompt, requests
+behind one system prompt) and for several new tokens a sequence (drafted
+tokens to be scored): the prefix is read once for the whole batch
+(scirs_b200/csrc/prefix_attention.cu).
+
 Reference parity: scirs2-neural/src/inference/paged_attention.rs:37-283
 (PagedAttentionConfig, PagedAttentionForward::forward(query, page_chain,
 pool)).
@@ -18,6 +24,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _ext
+from ..ops import kernels as K
 from .kv_cache import BlockManager, InferenceError, KvPagePool
 
 
@@ -68,12 +75,82 @@ class PagedAttentionForward:
             return out
         return paged_attention_reference(q, pool, block_tables, seq_lens, self._scale())
 
+    def forward_shared_prefix(self, q: torch.Tensor, pool: KvPagePool, block_tables: torch.Tensor,
+                              seq_lens: torch.Tensor, prefix_pages: torch.Tensor, prefix_len: int,
+                              q_lens: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the newest tokens of a batch whose first ``prefix_len`` tokens are the same.
+
+        q [B, H, HD], or [B, Q, H, HD] for up to Q tokens a sequence; block_tables int32
+        [B, max_pages], each sequence's whole chain; seq_lens int32 [B], its tokens with the newest
+        ones; prefix_pages int32, the pages of the prefix (it may end inside one); q_lens int32 [B],
+        how many of the Q queries a sequence has (default: all). Query t of a sequence stands at
+        position ``seq_len - q_len + t`` and sees the keys up to there. Rows past q_len, and
+        sequences of length 0, give zeros; a sequence with a query inside the prefix is read through
+        its own chain from the first key on. Every head_dim that is a multiple of 8 up to 128, any
+        number of query heads per cached head, any page size. bf16; the softmax and the sums are
+        kept in fp32. A captured graph keeps prefix_len, and reads the tables and lengths anew.
+        """
+        squeeze = q.dim() == 3
+        q4 = q.unsqueeze(1) if squeeze else q
+        c = pool.config
+        if q4.dim() != 4 or q4.shape[2:] != (self.config.num_heads, self.config.head_dim):
+            raise InferenceError("query shape does not match the configuration")
+        if self.config.num_heads % c.num_heads or self.config.head_dim != c.head_dim:
+            raise InferenceError("the pool's heads do not match the configuration")
+        if prefix_len < 0 or prefix_len > min(prefix_pages.numel(), block_tables.shape[-1]) * c.block_size:
+            raise InferenceError("prefix_len is longer than the prefix's pages or a chain")
+        if q.is_cuda:
+            out = _ext.kernels().paged_prefix_attention(q4.to(torch.bfloat16), pool.k, pool.v,
+                                                        block_tables.contiguous(), seq_lens.contiguous(),
+                                                        prefix_pages.contiguous(), int(prefix_len), q_lens,
+                                                        self._scale())
+            K._count(2)
+        else:
+            out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens,
+                                                    self._scale())
+        return out.squeeze(1) if squeeze else out
+
     def forward_manager(self, q: torch.Tensor, manager: BlockManager, seq_ids: list[int]):
         """Decode attention for the given sequences of a BlockManager."""
         manager.sync()
         rows = torch.tensor([manager.row_of(s) for s in seq_ids], dtype=torch.long, device=manager.block_tables.device)
         return self.forward_batch(q, manager.pool, manager.block_tables[rows].contiguous(),
                                   manager.seq_lens[rows].contiguous())
+
+    def forward_manager_shared(self, q: torch.Tensor, manager: BlockManager, seq_ids: list[int],
+                               q_lens: torch.Tensor | None = None):
+        """forward_shared_prefix for sequences of a BlockManager, over the pages that they share."""
+        manager.sync()
+        dev = manager.block_tables.device
+        pages, n = manager.shared_prefix(seq_ids)
+        rows = torch.tensor([manager.row_of(s) for s in seq_ids], dtype=torch.long, device=dev)
+        return self.forward_shared_prefix(q, manager.pool, manager.block_tables[rows], manager.seq_lens[rows],
+                                          torch.tensor(pages, dtype=torch.int32, device=dev), n, q_lens)
+
+
+def shared_prefix_attention_reference(q, pool: KvPagePool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens,
+                                      scale):
+    """fp32 PyTorch restatement of forward_shared_prefix (oracle); q [B, Q, H, HD]."""
+    B, Q, H, HD = q.shape
+    Hkv, bs = pool.config.num_heads, pool.config.block_size
+    G = H // Hkv
+    out = torch.zeros(B, Q, H, HD, dtype=torch.bfloat16, device=q.device)
+    for b in range(B):
+        n = min(max(int(seq_lens[b]), 0), block_tables.shape[1] * bs)
+        ql = Q if q_lens is None else min(max(int(q_lens[b]), 0), Q)
+        pos = torch.arange(n, device=pool.k.device)
+        pages = block_tables[b].long().to(pool.k.device)[pos // bs]
+        if n - ql + 1 >= prefix_len > 0:
+            head = pos < prefix_len
+            pages[head] = prefix_pages.long().to(pool.k.device)[pos[head] // bs]
+        k = pool.k[pages, pos % bs].float().repeat_interleave(G, dim=1)
+        v = pool.v[pages, pos % bs].float().repeat_interleave(G, dim=1)
+        for t in range(ql):
+            seen = n - ql + t + 1
+            if seen > 0:
+                s = torch.einsum("hd,thd->ht", q[b, t].float(), k[:seen]) * scale
+                out[b, t] = torch.einsum("ht,thd->hd", torch.softmax(s, dim=-1), v[:seen]).to(torch.bfloat16)
+    return out
 
 
 def paged_attention_reference(q, pool: KvPagePool, block_tables, seq_lens, scale):

@@ -11,6 +11,10 @@ zero floor the output distribution equals the target model's.
 Distributions are torch tensors (any device); sampling uses a Marsaglia
 xorshift64 generator so runs are reproducible from a seed.
 
+:func:`verify_drafts` does the same for a batch in one launch, from
+probabilities on the device and given random numbers
+(scirs_b200/csrc/draft_verify.cu).
+
 Reference parity: scirs2-neural/src/inference/speculative/types.rs:23-143
 (SpeculativeConfig, SpeculativeResult) and rejection_sampling.rs:46-667
 (Xorshift64, TokenDist, SpeculativeDecoder::rejection_sampling_step / decode).
@@ -18,8 +22,12 @@ Reference parity: scirs2-neural/src/inference/speculative/types.rs:23-143
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from typing import NamedTuple
 
 import torch
+
+from .. import _ext
+from ..ops import kernels as K
 
 
 @dataclass
@@ -101,6 +109,80 @@ class TokenDist:
     def prob(self, token: int, temperature: float) -> float:
         p = _probs(self.logits, temperature)
         return float(p[token]) if 0 <= token < p.numel() else 0.0
+
+
+class DraftVerification(NamedTuple):
+    accepted: torch.Tensor  # int32 [B]: how many drafted tokens are kept
+    tokens: torch.Tensor  # int64 [B, n + 1]: those, then the token that is drawn, then -1
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, draft_tokens: torch.Tensor,
+                  uniforms: torch.Tensor, draft_lens: torch.Tensor | None = None,
+                  acceptance_threshold: float = 0.0) -> DraftVerification:
+    """Keep or replace the drafted tokens of a batch.
+
+    target_probs [B, n + 1, V] holds the target's probabilities at each drafted token's place and at
+    the one behind the last, draft_probs [B, n, V] the draft's (None: the draft is certain of its
+    tokens, as a greedy or n-gram draft is); fp32, bf16 or fp16 with contiguous rows, both of one type.
+    draft_tokens int64 [B, n]; uniforms fp32 [B, n + 1] in [0, 1); draft_lens int32 [B] says how many
+    drafts a sequence has (default: n).
+
+    Draft x_i is kept while u_i q_i(x_i) < p_i(x_i), or u_i < acceptance_threshold (a draft of
+    probability 0: while p_i(x_i) > 0; one outside the vocabulary: never). At the first place that is
+    not kept one token is drawn from max(p - q, 0), or from p where that is zero everywhere, and from
+    the last p where all are kept: the first token whose cumulative weight exceeds u_n times the
+    total. The weights need not sum to 1; negative, infinite and NaN ones count as zero, and -1 is
+    returned in the token's place where nothing is left. Products and sums are formed in 64 bits."""
+    t, d = target_probs, draft_probs
+    if t.dim() != 3 or t.shape[1] < 1 or t.shape[2] < 1:
+        raise ValueError("target probabilities must be [B, n + 1, V]")
+    B, n, V = t.shape[0], t.shape[1] - 1, t.shape[2]
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("probabilities must be fp32, bf16 or fp16")
+    if d is not None and (d.shape != (B, n, V) or d.dtype != t.dtype or d.device != t.device):
+        raise ValueError(f"draft probabilities must be [{B}, {n}, {V}], typed and placed as the target's")
+    if draft_tokens.shape != (B, n) or draft_tokens.dtype != torch.int64:
+        raise ValueError(f"draft tokens must be int64 [{B}, {n}]")
+    if uniforms.shape != (B, n + 1) or uniforms.dtype != torch.float32:
+        raise ValueError(f"uniforms must be fp32 [{B}, {n + 1}]")
+    if draft_lens is not None and (draft_lens.shape != (B,) or draft_lens.dtype != torch.int32):
+        raise ValueError(f"draft lengths must be int32 [{B}]")
+    if t.is_cuda:
+        t = t if V == 1 or t.stride(2) == 1 else t.contiguous()
+        if d is not None and V > 1 and d.stride(2) != 1:
+            d = d.contiguous()
+        out = _ext.kernels().draft_verify(t, d, draft_tokens.contiguous(), uniforms.contiguous(),
+                                          None if draft_lens is None else draft_lens.contiguous(),
+                                          float(acceptance_threshold))
+        K._count(1)
+        return DraftVerification(*out)
+    accepted, tokens = torch.zeros(B, dtype=torch.int32), torch.full((B, n + 1), -1, dtype=torch.int64)
+    for b in range(B):
+        m, kept, q = n if draft_lens is None else min(max(int(draft_lens[b]), 0), n), 0, None
+        while kept < m:
+            x, u = int(draft_tokens[b, kept]), float(uniforms[b, kept])
+            q = torch.zeros(V, dtype=torch.float64)
+            if d is not None:
+                q = d[b, kept].double()
+            elif 0 <= x < V:
+                q[x] = 1.0
+            if not 0 <= x < V:
+                break
+            px, qx = float(t[b, kept, x]), float(q[x])
+            if not (px > 0.0 if qx <= 0.0 else u < 1.0 and (u * qx < px or u < acceptance_threshold)):
+                break
+            tokens[b, kept] = x
+            kept += 1
+        accepted[b] = kept
+        p = t[b, kept].double()
+        for w in ([p - q, p] if kept < m else [p]):
+            w = torch.where((w > 0) & torch.isfinite(w), w, torch.zeros_like(w))
+            if float(w.sum()) > 0.0:
+                c = torch.cumsum(w, 0)
+                past = torch.nonzero((c > float(uniforms[b, n]) * c[-1]) & (w > 0))
+                tokens[b, kept] = int(past[0] if len(past) else torch.nonzero(w > 0)[-1])
+                break
+    return DraftVerification(accepted, tokens)
 
 
 class SpeculativeDecoder:

@@ -53,6 +53,9 @@ ext_modules = [
                 "attention_fwd_sm100.cu",
                 "attention_bwd_sm100.cu",
                 "paged_attention.cu",
+                "prefix_attention.cu",
+                "page_copy.cu",
+                "draft_verify.cu",
                 "conv.cu",
                 "elementwise.cu",
                 "rnn.cu",
