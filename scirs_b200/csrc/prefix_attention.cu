@@ -26,64 +26,11 @@
 //
 // Reference parity: scirs2-neural/src/inference/paged_attention.rs:113-283 (one query over one page
 // chain), block_manager.rs:196-280 (SharedPrefixCache: the pages a prefix's sequences share).
-#include "host_common.h"
+#include "prefix_attention.cuh"
 
 namespace scirs {
 namespace prefix {
 
-using bf16 = __nv_bfloat16;
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kTile = 16;  // keys per step of a warp
-constexpr int kStages = 3;
-constexpr int kStep = kTile * kWarps;  // keys per step of a CTA: split lengths are multiples
-
-struct Params {
-  const bf16 *q, *k, *v;
-  bf16* out;
-  const int *tables, *lens, *qlens, *pages;  // qlens may be null: Q each
-  float *part_o, *part_ml;                   // [B Q H, slots, HD], [B Q H, slots, 2]
-  long q_sb, q_st, q_sh;                     // element strides of q
-  int table_stride, max_pages, num_pages;
-  int B, Q, H, Hkv, G, HD, bs;
-  int L;                // tokens of the prefix
-  int P, per_p, rt_p;   // prefix: splits, keys a split, row tiles
-  int T, rt_t;          // tails: splits, row tiles of a sequence
-  float scale_log2;
-  DevStatus* st;
-};
-
-struct Seq {
-  int len, ql, start;  // tokens, queries, first key that is read through the sequence's own chain
-};
-
-__device__ __forceinline__ Seq seq_of(const Params& p, int b, bool report = false) {
-  Seq s;
-  s.len = max(p.lens[b], 0);
-  if ((long)s.len > (long)p.max_pages * p.bs) {  // not addressable
-    if (report) report_status(p.st, kStBounds, 95, (unsigned)s.len);
-    s.len = p.max_pages * p.bs;
-  }
-  s.ql = p.qlens != nullptr ? min(max(p.qlens[b], 0), p.Q) : p.Q;
-  if (s.ql == 0) s.len = 0;
-  s.start = s.len - s.ql + 1 >= p.L ? p.L : 0;
-  return s;
-}
-
-// Keys of a split of a sequence's tail: an even share, in whole steps.
-__device__ __forceinline__ int tail_share(const Params& p, const Seq& s) {
-  const int n = max(s.len - s.start, 0);
-  return ((n + p.T - 1) / p.T + kStep - 1) / kStep * kStep;
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {
-  const int n = full ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -131,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) item_kernel(const Params p) {
 
   // ---- which rows against which keys
   int i = blockIdx.x;
-  const int prefix_items = p.P * p.Hkv * p.rt_p;
+  const int prefix_items = p.P * p.Hkv * p.rt_p;  // none when tcgen05 takes the prefix
   const bool is_prefix = i < prefix_items;
   int hk, r0, r_end, k0, k1, slot, max_pages;
   const int* pages;
@@ -215,19 +162,11 @@ __global__ void __launch_bounds__(kThreads) item_kernel(const Params p) {
   }
   const int first = k0 + warp * kTile;
   const int steps = first < k1 ? (k1 - first + kStep - 1) / kStep : 0;
-  const long head_off = (long)hk * p.HD, row_elems = (long)p.Hkv * p.HD;
   uint32_t valid[kStages - 1];  // of the steps on their way: the keys that are read (bit = key)
 
   auto load = [&](int j, int s) -> uint32_t {
     const int key = first + j * kStep + lane;  // lanes 0-15 look their key's page up
-    long off = -1;
-    if (lane < kTile && key < k1) {
-      const int pi = key / p.bs;
-      if (pi < max_pages) {
-        const int page = pages[pi];
-        if (input_in_range(page, p.num_pages, p.st, 96)) off = ((long)page * p.bs + key % p.bs) * row_elems + head_off;
-      }
-    }
+    const long off = lane < kTile && key < k1 ? pool_row(p, pages, max_pages, key, hk) : -1;
     constexpr int RPI = 32 / (HDP / 8);  // rows per instruction
     const int c = lane % (HDP / 8);
 #pragma unroll
@@ -434,18 +373,28 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const int t = (int)(row / p.H % p.Q);
   const Seq s = seq_of(p, b);
   const int share = tail_share(p, s), n = max(s.len - s.start, 0);
-  // the slots that hold parts of this row: the prefix's, if the sequence reads it there, and its tail's
-  const int s0 = s.start == p.L ? 0 : p.P;
-  const int s1 = t < s.ql && n > 0 ? p.P + (n + share - 1) / share : (t < s.ql ? p.P : s0);
+  // the slots that hold parts of this row: the prefix's, if the sequence takes part in it, and its tail's
+  int np = 0;  // prefix slots
+  if (t < s.ql && s.start == p.L) {
+    np = p.P;
+    if (p.tc_share > 0) {
+      // the CTAs whose blocks meet the row tile's
+      const int h = (int)(row % p.H), hk = h / p.G, r = (b * p.Q + t) * p.G + h % p.G;
+      const long first = ((long)hk * p.tc_tiles + r / p.tc_rows) * p.tc_blocks;
+      np = (int)((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
+    }
+  }
+  const int nt = t < s.ql && n > 0 ? (n + share - 1) / share : 0;  // tail slots
   const int slots = p.P + p.T;
   const float* ml = p.part_ml + row * slots * 2;
   const float* po = p.part_o + row * slots * p.HD;
   float m = -INFINITY;
-  for (int i = s0 + lane; i < s1; i += 32) m = fmaxf(m, ml[2 * i]);
+  for (int j = lane; j < np + nt; j += 32) m = fmaxf(m, ml[2 * (j < np ? j : p.P + j - np)]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int i = s0; i < s1; ++i) {
+  for (int j = 0; j < np + nt; ++j) {
+    const int i = j < np ? j : p.P + j - np;
     const float f = ex2_fast(ml[2 * i] - ref);
     if (f == 0.f) continue;
     den += f * ml[2 * i + 1];
@@ -463,6 +412,8 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 // q [B, Q, H, HD] bf16 (inner dimension contiguous) -> [B, Q, H, HD] bf16. Pools [num_pages, block_size,
 // Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
+constexpr int64_t kTcRows = 32, kTcKeys = 256;
+
 torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
                                      torch::Tensor lens, torch::Tensor pages, int64_t L,
                                      c10::optional<torch::Tensor> qlens, double scale) {
@@ -500,8 +451,8 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   c10::cuda::CUDAGuard guard(q.get_device());
   auto out = at::empty({B, Q, H, HD}, q.options());
   if (out.numel() == 0) return out;
-  if (q.stride(3) != 1 || q.stride(0) % 2 || q.stride(1) % 2 || q.stride(2) % 2 ||
-      reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 != 0)
+  if (q.stride(3) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || q.stride(2) % 8 ||
+      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
     q = q.clone(at::MemoryFormat::Contiguous);  // (contiguous() would keep a contiguous tensor at an odd offset)
   prefix::Params p{};
   p.q = reinterpret_cast<const prefix::bf16*>(q.data_ptr());
@@ -529,23 +480,30 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   p.st = status_ptr(q.get_device());
 
   const int64_t seq_rows = Q * p.G, rows = B * seq_rows;
-  const int mt = std::max(L > 0 ? rows : 0, seq_rows) > 16 ? 2 : 1;
-  p.rt_p = L > 0 ? (int)((rows + 16 * mt - 1) / (16 * mt)) : 0;
+  const int sms = num_sms(q.get_device());
+  const bool tc = L >= kTcKeys && rows > kTcRows;
+  const int mt = std::max(L > 0 && !tc ? rows : 0, seq_rows) > 16 ? 2 : 1;
+  p.rt_p = L > 0 && !tc ? (int)((rows + 16 * mt - 1) / (16 * mt)) : 0;
   p.rt_t = (int)((seq_rows + 16 * mt - 1) / (16 * mt));
   // equal shares of keys for about four items per SM
   const int64_t span = max_pages * bs - L;
   const int64_t work = Hkv * (p.rt_p * L + B * p.rt_t * span);
-  int64_t unit = work / (4LL * num_sms(q.get_device()));
+  int64_t unit = work / (4LL * sms);
   unit = std::max<int64_t>(256, (unit + prefix::kStep - 1) / prefix::kStep * prefix::kStep);
-  p.P = (int)((L + unit - 1) / unit);
+  p.P = tc ? 0 : (int)((L + unit - 1) / unit);
   p.per_p = (int)unit;
   p.T = (int)std::max<int64_t>(1, (span + unit - 1) / unit);
+  if (tc) prefix::plan_prefix_tc(p, sms);
   const int slots = p.P + p.T;
   auto part_o = at::empty({B * Q * H, slots, HD}, q.options().dtype(at::kFloat));
   auto part_ml = at::empty({B * Q * H, slots, 2}, q.options().dtype(at::kFloat));
   p.part_o = part_o.data_ptr<float>();
   p.part_ml = part_ml.data_ptr<float>();
   const int64_t items = Hkv * ((int64_t)p.rt_p * p.P + B * p.rt_t * p.T);
+  if (tc) {
+    prefix::launch_prefix_tc(p, cur_stream());
+    SCIRS_CHECK_LAUNCH();
+  }
   TORCH_CHECK(items < (1LL << 31), "paged attention: too large");
   auto st = cur_stream();
 #define SCIRS_ITEMS(HDP_, MT_)                                              \

@@ -1,0 +1,433 @@
+// The shared prefix on tcgen05: all rows of the batch that share a cached head, in tiles, against the
+// prefix's keys in blocks of 128.
+//
+// 512 threads, one CTA per SM:
+//   warp 0        issues the MMAs (one thread) and owns TMEM
+//   warps 4-7     producers: K and V blocks go through a ring of slots; unit 2 j is K of block j, 2 j + 1
+//                 its V, and unit u belongs to warp 4 + u % 4, which copies it with cp.async (16 bytes a
+//                 lane, any page size, written in the 128-byte swizzle that the MMA reads), waits for its
+//                 own copies, makes them visible to the asynchronous proxy and signals the slot full
+//   warps 8-15    two softmax warpgroups, a thread per row: read the row's 128 scores from TMEM, raise the
+//                 running maximum only when it grew by more than 2^8 (then O is rescaled in TMEM), write P
+//                 back as packed bf16 over the scores
+// S_t at TMEM columns [128 t, +128) (P_t aliases its first half), O_t at [256 + HDP t, + HDP). MMAs of one
+// thread complete in order, so S_t of the next block may take the columns that P V_t reads, and S_t being
+// full implies that P V_t before it is in O_t.
+//
+// Two schedules (template STREAMS):
+//   1: a row tile is 256 rows, tile t its 128-row half; both use every key block (many rows: a K/V block is
+//      read once for 256 rows, and one half's softmax runs during the other half's MMAs)
+//   2: a row tile is 128 rows; tile t takes every other key block of the same rows (few rows: two
+//      independent chains keep the loads and the tensor core busy), and writes a part of its own
+//
+// Work is laid out evenly: the blocks of all row tiles end to end are cut into equal shares, one per CTA,
+// so a CTA may finish one row tile and begin the next; its part of a row tile goes to the slot given by how
+// many CTAs before it met that tile. Every wait is bounded (common.cuh).
+//
+// Reference parity: scirs2-neural/src/inference/paged_attention.rs:113-283.
+#include "prefix_attention.cuh"
+
+namespace scirs {
+namespace prefix {
+
+constexpr int kTcThreads = 512;
+constexpr int kBlk = 128;  // keys of a block, rows of a tile
+// warpgroups: MMA, producers, two of softmax; 512 x 128 registers at launch
+constexpr int kRegsMma = 48, kRegsLoad = 56, kRegsSoftmax = 200;
+static_assert(kRegsMma + kRegsLoad + 2 * kRegsSoftmax <= 4 * 128, "register split exceeds the launch");
+constexpr float kRaise = 8.f;  // raise the reference maximum only past 2^8
+
+template <int HDP>
+struct Tc {
+  static constexpr int TILE = kBlk * HDP * 2;  // a Q tile, or K or V of a block
+  static constexpr int NS = HDP == 64 ? 8 : 4;  // ring slots
+  static constexpr int OFF_Q = 0;               // two tiles
+  static constexpr int OFF_RING = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_RING + NS * TILE;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr uint32_t IDESC_S = umma_idesc_bf16(kBlk, kBlk, 0, 0);
+  static constexpr uint32_t IDESC_O = umma_idesc_bf16(kBlk, HDP, 0, 1);
+};
+
+// A CTA's part of a row tile: blocks [j0, j0 + n).
+struct TcItem {
+  int hk, r0, j0, n, slot, tiles;
+};
+
+template <int STREAMS>
+__device__ __forceinline__ TcItem tc_item(const Params& p, long u, long end) {
+  TcItem i;
+  const long g = u / p.tc_blocks;
+  i.hk = (int)(g / p.tc_tiles);
+  i.r0 = (int)(g % p.tc_tiles) * p.tc_rows;
+  i.j0 = (int)(u % p.tc_blocks);
+  i.n = (int)min((long)(p.tc_blocks - i.j0), end - u);
+  i.slot = (int)(blockIdx.x - g * p.tc_blocks / p.tc_share) * STREAMS;
+  i.tiles = STREAMS == 2 ? min(2, i.n) : (i.r0 + kBlk < p.B * p.Q * p.G ? 2 : 1);
+  return i;
+}
+
+template <int HDP, int STREAMS>
+__global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p) {
+  using C = Tc<HDP>;
+  constexpr int NS = C::NS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [NS]
+  uint64_t* empty = full + NS;                                      // [NS]
+  uint64_t* s_full = empty + NS;                                    // [2]
+  uint64_t* p_full = s_full + 2;                                    // [2]
+  uint64_t* o_full = p_full + 2;                                    // [2]
+  uint64_t* q_full = o_full + 2;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* drain = q_empty + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = p.HD / 8;  // 16-byte chunks of a row; the rest of a padded row stays zero
+  const long u_begin = blockIdx.x * p.tc_share;
+  const long u_end = min(u_begin + p.tc_share, (long)p.Hkv * p.tc_tiles * p.tc_blocks);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(q_full, STREAMS == 2 ? 4 : 8);
+    mbar_init(q_empty, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  if (chunks < HDP / 8) {
+    for (int i = threadIdx.x; i < C::OFF_BAR / 16; i += kTcThreads)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp < 4) {
+    setmaxnreg_dec<kRegsMma>();
+    if (warp == 0 && lane == 0) {
+      // -------------------------------------------------------------- MMA
+      const uint32_t q_addr = smem_u32(smem + C::OFF_Q), ring = smem_u32(smem + C::OFF_RING);
+      int blk = 0;           // blocks of earlier items: unit 2 (blk + j) is K of block j
+      int done[2] = {0, 0};  // phases of p_full
+      bool ok = true;
+      auto wait_unit = [&](int u) -> bool {
+        if (!mbar_wait(&full[u % NS], (u / NS) & 1, p.st, 100, abort_flag)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto issue_s = [&](int t, int j) {
+        const uint32_t ka = ring + ((2 * (blk + j)) % NS) * C::TILE;
+        const uint32_t qa = q_addr + (STREAMS == 2 ? 0 : t * C::TILE);
+#pragma unroll
+        for (int kk = 0; kk < HDP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kBlk * 128) + (kk & 3) * 32;
+          tc_mma_f16_ss(tmem + t * kBlk, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
+                        C::IDESC_S, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int t, int j, bool first) {
+        const uint32_t va = ring + ((2 * (blk + j) + 1) % NS) * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < kBlk / 16; ++kk)
+          // A = P_t from TMEM (16 keys = 8 packed columns a step), B = V [keys][HDP] MN-major
+          tc_mma_f16_ts(tmem + 2 * kBlk + t * HDP, tmem + t * kBlk + kk * 8,
+                        umma_desc_sw128(va + kk * 2048, kBlk * 128, 1024), C::IDESC_O, !first || kk > 0 ? 1u : 0u);
+      };
+      auto release = [&](int u) { tc_commit(&empty[u % NS]); };
+      int ii = 0;
+      for (long u = u_begin; u < u_end && ok; ++ii) {
+        const TcItem I = tc_item<STREAMS>(p, u, u_end);
+        if (!mbar_wait(q_full, ii & 1, p.st, 101, abort_flag)) break;
+        tc_fence_after();
+        if (STREAMS == 1) {
+          ok = wait_unit(2 * blk);
+          if (!ok) break;
+          for (int t = 0; t < I.tiles; ++t) issue_s(t, 0);
+          release(2 * blk);
+          if (I.n == 1) tc_commit(q_empty);
+          for (int j = 0; j < I.n && ok; ++j) {
+            for (int t = 0; t < I.tiles; ++t) {
+              ok = ok && mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag);
+              if (ok && t == 0) ok = wait_unit(2 * (blk + j) + 1);
+              if (!ok) break;
+              ++done[t];
+              tc_fence_after();
+              issue_pv(t, j, j == 0);
+              if (j + 1 < I.n) {
+                if (t == 0) ok = wait_unit(2 * (blk + j + 1));
+                if (!ok) break;
+                issue_s(t, j + 1);
+              } else {
+                tc_commit(&o_full[t]);
+              }
+            }
+            if (!ok) break;
+            release(2 * (blk + j) + 1);
+            if (j + 1 < I.n) release(2 * (blk + j + 1));
+            if (j == I.n - 2) tc_commit(q_empty);
+          }
+        } else {
+          for (int t = 0; t < I.tiles && ok; ++t) {
+            ok = wait_unit(2 * (blk + t));
+            if (!ok) break;
+            issue_s(t, t);
+            release(2 * (blk + t));
+          }
+          if (ok && I.n <= 2) tc_commit(q_empty);
+          for (int j = 0; j < I.n && ok; ++j) {
+            const int t = j & 1;
+            ok = mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag) && wait_unit(2 * (blk + j) + 1);
+            if (!ok) break;
+            ++done[t];
+            tc_fence_after();
+            issue_pv(t, j, j < 2);
+            release(2 * (blk + j) + 1);
+            if (j + 2 < I.n) {
+              ok = wait_unit(2 * (blk + j + 2));
+              if (!ok) break;
+              issue_s(t, j + 2);
+              release(2 * (blk + j + 2));
+              if (j + 3 == I.n) tc_commit(q_empty);
+            } else {
+              tc_commit(&o_full[t]);
+            }
+          }
+        }
+        blk += I.n;
+        u += I.n;
+      }
+      tc_commit(drain);
+      mbar_wait(drain, 0, nullptr, 0, nullptr);
+    }
+  } else if (warp < 8) {
+    setmaxnreg_dec<kRegsLoad>();
+    // ---------------------------------------------------------------- producers
+    const int w = warp - 4;
+    constexpr int CPR = HDP / 8, RPI = 32 / CPR;  // chunks of a row, rows an instruction
+    const int c = lane % CPR;
+    const bf16* src = (w & 1) ? p.v : p.k;
+    const uint32_t ring = smem_u32(smem + C::OFF_RING);
+    const int max_pages = (p.L + p.bs - 1) / p.bs;
+    int blk = 0;
+    bool ok = true;
+    for (long u = u_begin; u < u_end && ok;) {
+      const TcItem I = tc_item<STREAMS>(p, u, u_end);
+      for (int j = 0; j < I.n; ++j) {
+        const int unit = 2 * (blk + j) + (w & 1);
+        if ((unit & 3) != w) continue;
+        // this lane looks four keys' rows up
+        long row[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = (I.j0 + j) * kBlk + i * 32 + lane;
+          row[i] = key < p.L ? pool_row(p, p.pages, max_pages, key, I.hk) : -1;
+        }
+        if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t slot = ring + (unit % NS) * C::TILE + (c >> 3) * (kBlk * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll 8
+          for (int k = 0; k < 32; k += RPI) {
+            const int r = k + lane / CPR;
+            const long e = __shfl_sync(0xffffffffu, row[i], r);
+            if (c < chunks)
+              cp_async16(slot + (i * 32 + r) * 128 + (((c ^ r) & 7) << 4), src + (e < 0 ? 0 : e) + c * 8, e >= 0);
+          }
+        cp_commit();
+        cp_wait<0>();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[unit % NS]);
+      }
+      blk += I.n;
+      u += I.n;
+    }
+  } else {
+    setmaxnreg_inc<kRegsSoftmax>();
+    // ---------------------------------------------------------------- softmax
+    const int t = (warp - 8) >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t s_base = tmem + lane_off + t * kBlk;
+    const uint32_t o_base = tmem + lane_off + 2 * kBlk + t * HDP;
+    const int slots = p.P + p.T;
+    int cnt = 0, fin = 0, ii = 0;  // phases of s_full and o_full
+    bool ok = true;
+    for (long u = u_begin; u < u_end && ok; ++ii) {
+      const TcItem I = tc_item<STREAMS>(p, u, u_end);
+      const int gr = I.r0 + (STREAMS == 2 ? 0 : t * kBlk) + r;
+      const bf16* q = prefix_query(p, gr, I.hk);
+      if (STREAMS == 1 || t == 0) {
+        // Q of this row (zeros for a row that takes no part)
+        if (!mbar_wait(q_empty, (ii & 1) ^ 1, p.st, 104, abort_flag)) break;
+        uint8_t* dst = smem + C::OFF_Q + t * C::TILE + r * 128;
+#pragma unroll 4
+        for (int c = 0; c < chunks; ++c)
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBlk * 128) + (((c ^ r) & 7) << 4)) =
+              q != nullptr ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      const int n = t >= I.tiles ? 0 : (STREAMS == 2 ? (I.n - t + 1) / 2 : I.n);
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < n && ok; ++j, ++cnt) {
+        if (!mbar_wait(&s_full[t], cnt & 1, p.st, 105, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float sv[kBlk];
+        {
+          uint32_t* x = reinterpret_cast<uint32_t*>(sv);
+#pragma unroll
+          for (int c = 0; c < kBlk; c += 32) tmem_ld_32x32b_x32(s_base + c, x + c);
+          tc_wait_ld();
+        }
+        const int left = p.L - (I.j0 + (STREAMS == 2 ? 2 * j + t : j)) * kBlk;
+        if (left < kBlk) {
+#pragma unroll
+          for (int e = 0; e < kBlk; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
+        }
+        float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+        for (int e = 4; e < kBlk; e += 8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            m4[i] = e + 4 + i < kBlk ? fmaxf(fmaxf(m4[i], sv[e + i]), sv[e + 4 + i]) : fmaxf(m4[i], sv[e + i]);
+        }
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+        const bool raise = mx > m_ref + kRaise;
+        float alpha = 1.f;
+        if (raise) {
+          alpha = ex2_fast(m_ref - mx);  // 0 before the first block
+          m_ref = mx;
+          l *= alpha;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+          for (int c = 0; c < HDP; c += 32) {
+            uint32_t ov[32];
+            tmem_ld_32x32b_x32(o_base + c, ov);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+            tmem_st_32x32b_x16(o_base + c, ov);
+            tmem_st_32x32b_x16(o_base + c + 16, ov + 16);
+          }
+          tc_wait_st();
+        }
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(-ref, -ref);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < kBlk; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(sv[c + e], sv[c + e + 1]), sc2, nref2), x0, x1);
+            x0 = ex2_fast(x0);
+            x1 = ex2_fast(x1);
+            sum2[(e >> 1) & 1] = f2_add(sum2[(e >> 1) & 1], f2_pack(x0, x1));
+            pk[e >> 1] = pack_bf16x2(x0, x1);
+          }
+          tmem_st_32x32b_x16(s_base + (c >> 1), pk);
+        }
+        float l0, l1;
+        f2_unpack(f2_add(sum2[0], sum2[1]), l0, l1);
+        l += l0 + l1;
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // this CTA's part of the row
+      const int bt = gr / p.G;
+      const long at = ((long)bt * p.H + I.hk * p.G + gr % p.G) * slots + I.slot + (STREAMS == 2 ? t : 0);
+      const bool live = q != nullptr && n > 0;
+      if (n > 0) {
+        if (!mbar_wait(&o_full[t], fin & 1, p.st, 106, abort_flag)) break;
+        ++fin;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < HDP; c += 32) {
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(o_base + c, ov);
+          tc_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < p.HD)
+                *reinterpret_cast<uint4*>(p.part_o + at * p.HD + c + e) = make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      if (q != nullptr) {
+        p.part_ml[at * 2] = live ? m_ref : -INFINITY;
+        p.part_ml[at * 2 + 1] = live ? l : 0.f;
+      }
+      u += I.n;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+void plan_prefix_tc(Params& p, int sms) {
+  const int rows = p.B * p.Q * p.G;
+  p.tc_streams = rows > kBlk ? 1 : 2;
+  p.tc_rows = rows > kBlk ? 2 * kBlk : kBlk;
+  p.tc_tiles = (rows + p.tc_rows - 1) / p.tc_rows;
+  p.tc_blocks = (p.L + kBlk - 1) / kBlk;
+  const long units = (long)p.Hkv * p.tc_tiles * p.tc_blocks;
+  p.tc_share = std::max<long>(2, (units + sms - 1) / sms);
+  p.P = (int)((p.tc_blocks - 1) / p.tc_share + 2) * p.tc_streams;
+}
+
+template <int HDP, int STREAMS>
+static void launch_tc(const Params& p, cudaStream_t st) {
+  auto kern = prefix_tc_kernel<HDP, STREAMS>;
+  set_max_smem((const void*)kern, Tc<HDP>::SMEM);
+  const long units = (long)p.Hkv * p.tc_tiles * p.tc_blocks;
+  kern<<<(unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st>>>(p);
+}
+
+void launch_prefix_tc(const Params& p, cudaStream_t st) {
+  if (p.HD <= 64) {
+    p.tc_streams == 1 ? launch_tc<64, 1>(p, st) : launch_tc<64, 2>(p, st);
+  } else {
+    p.tc_streams == 1 ? launch_tc<128, 1>(p, st) : launch_tc<128, 2>(p, st);
+  }
+}
+
+}  // namespace prefix
+}  // namespace scirs

@@ -54,6 +54,7 @@ ext_modules = [
                 "attention_bwd_sm100.cu",
                 "paged_attention.cu",
                 "prefix_attention.cu",
+                "prefix_attention_sm100.cu",
                 "page_copy.cu",
                 "draft_verify.cu",
                 "conv.cu",

@@ -114,6 +114,15 @@ CASES = [
     pytest.param([257 + 3 * i for i in range(40)], 1, 2, 4, 128, 16, 256, None, id="forty_sequences"),
     pytest.param([400 + i for i in range(70)], 2, 1, 4, 64, 16, 397, [1 + i % 2 for i in range(70)], id="seventy_by_two"),
     pytest.param([1500 + 7 * i for i in range(33)], 1, 2, 8, 128, 16, 1493, None, id="three_row_tiles"),
+    # 33 to 128 rows a cached head, and more, against prefixes of two blocks and more
+    pytest.param([260, 270, 0, 300, 259], 1, 2, 8, 128, 16, 259, None, id="forty_rows"),
+    pytest.param([2100 + i for i in range(25)], 4, 1, 1, 64, 24, 2100 - 4, [1 + i % 4 for i in range(25)], id="hundred_rows"),
+    pytest.param([700, 30, 701, 0, 699] * 5, 2, 3, 5, 96, 32, 690, [2, 1, 0, 2, 1] * 5, id="rows_that_take_no_part"),
+    pytest.param([1025] * 20, 1, 1, 2, 40, 5, 1024, None, id="tc_head_dim_40_pages_of_five"),
+    pytest.param([257 + i for i in range(64)], 1, 1, 2, 128, 16, 257, None, id="tails_of_none_128_rows"),
+    pytest.param([520 + i for i in range(129)], 1, 1, 1, 64, 16, 512, None, id="129_rows"),
+    pytest.param([4000 + i for i in range(6)], 1, 16, 7, 64, 128, 3999, None, id="sixteen_heads"),
+    pytest.param([5000 + 3 * i for i in range(40)], 1, 1, 16, 128, 16, 4990, None, id="640_rows_long"),
 ]
 
 
