@@ -76,4 +76,22 @@ CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t i
   return m;
 }
 
+CUtensorMap make_tmap_bf16(const void* base, int rank, const uint64_t* extents, const uint64_t* strides,
+                           const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  CUtensorMap m;
+  cuuint64_t dims[5], str[4];
+  cuuint32_t bx[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = extents[i];
+    bx[i] = box[i];
+    one[i] = 1;
+    if (i + 1 < rank) str[i] = strides[i];
+  }
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, str, bx, one,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", num((int)r));
+  return m;
+}
+
 }  // namespace scirs

@@ -45,6 +45,11 @@ CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t i
                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                          CUtensorMapSwizzle swizzle);
 
+// Encode a tiled bf16 map of up to 5 dimensions: extents and box innermost first, strides (bytes) of the
+// dimensions behind the first.
+CUtensorMap make_tmap_bf16(const void* base, int rank, const uint64_t* extents, const uint64_t* strides,
+                           const uint32_t* box, CUtensorMapSwizzle swizzle);
+
 inline std::string num(int64_t v) { return std::to_string(v); }
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }

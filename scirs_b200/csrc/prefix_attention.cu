@@ -364,11 +364,12 @@ __global__ void __launch_bounds__(kThreads) item_kernel(const Params p) {
   }
 }
 
-// One warp per output row.
+// One CTA per output row; its warps take every fourth part.
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
-  const long row = blockIdx.x * 4L + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (long)p.B * p.Q * p.H) return;
+  const long row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float4 acc_s[4][32];
+  __shared__ float den_s[4];
   const int b = (int)(row / ((long)p.Q * p.H));
   const int t = (int)(row / p.H % p.Q);
   const Seq s = seq_of(p, b);
@@ -380,31 +381,55 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
     if (p.tc_share > 0) {
       // the CTAs whose blocks meet the row tile's
       const int h = (int)(row % p.H), hk = h / p.G, r = (b * p.Q + t) * p.G + h % p.G;
-      const long first = ((long)hk * p.tc_tiles + r / p.tc_rows) * p.tc_blocks;
-      np = (int)((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
+      const int first = (hk * p.tc_tiles + r / p.tc_rows) * p.tc_blocks;
+      np = ((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
     }
   }
   const int nt = t < s.ql && n > 0 ? (n + share - 1) / share : 0;  // tail slots
   const int slots = p.P + p.T;
   const float* ml = p.part_ml + row * slots * 2;
   const float* po = p.part_o + row * slots * p.HD;
+  const auto slot_of = [&](int j) { return j < np ? j : p.P + j - np; };
   float m = -INFINITY;
-  for (int j = lane; j < np + nt; j += 32) m = fmaxf(m, ml[2 * (j < np ? j : p.P + j - np)]);
+  for (int j = lane; j < np + nt; j += 32) m = fmaxf(m, ml[2 * slot_of(j)]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
-  float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-  for (int j = 0; j < np + nt; ++j) {
-    const int i = j < np ? j : p.P + j - np;
-    const float f = ex2_fast(ml[2 * i] - ref);
-    if (f == 0.f) continue;
-    den += f * ml[2 * i + 1];
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < p.HD) num[e] += f * po[(long)i * p.HD + lane + 32 * e];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+  const bool on = 4 * lane < p.HD;
+#pragma unroll 4
+  for (int j = warp; j < np + nt; j += 4) {
+    const int i = slot_of(j);
+    const float2 v = *reinterpret_cast<const float2*>(ml + 2 * i);
+    const float4 o = on ? *reinterpret_cast<const float4*>(po + (long)i * p.HD + 4 * lane) : acc;
+    const float w = ex2_fast(v.x - ref);
+    if (w != 0.f) {  // (a part without keys holds nothing)
+      den += w * v.y;
+      acc.x += w * o.x;
+      acc.y += w * o.y;
+      acc.z += w * o.z;
+      acc.w += w * o.w;
+    }
   }
+  acc_s[warp][lane] = acc;
+  if (lane == 0) den_s[warp] = den;
+  __syncthreads();
+  if (warp != 0 || !on) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < p.HD) p.out[row * p.HD + lane + 32 * e] = __float2bfloat16(den == 0.f ? 0.f : num[e] / den);
+  for (int w = 1; w < 4; ++w) {
+    const float4 o = acc_s[w][lane];
+    acc.x += o.x;
+    acc.y += o.y;
+    acc.z += o.z;
+    acc.w += o.w;
+    den += den_s[w];
+  }
+  uint2 out = make_uint2(0u, 0u);
+  if (den != 0.f) {
+    const float inv = 1.f / den;
+    out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  }
+  *reinterpret_cast<uint2*>(p.out + row * p.HD + 4 * lane) = out;
 }
 
 }  // namespace prefix
@@ -445,6 +470,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   TORCH_CHECK(tables.dim() == 2 && tables.size(0) == B && lens.numel() == B && (!has_ql || qlens->numel() == B),
               "one table row, length and query length per sequence");
   const int64_t max_pages = tables.size(1);
+  TORCH_CHECK(num_pages > 0 || L == 0, "an empty pool holds no prefix");
   TORCH_CHECK(L >= 0 && L <= pages.numel() * bs && L <= max_pages * bs, "a prefix of ", num(L),
               " tokens is longer than its pages or than a chain");
   TORCH_CHECK(max_pages * bs < (1LL << 30) && B * Q * H < (1LL << 30), "paged attention: too large");
@@ -519,7 +545,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   }
 #undef SCIRS_ITEMS
   SCIRS_CHECK_LAUNCH();
-  prefix::combine_kernel<<<(unsigned)((B * Q * H + 3) / 4), 128, 0, st>>>(p);
+  prefix::combine_kernel<<<(unsigned)(B * Q * H), 128, 0, st>>>(p);
   SCIRS_CHECK_LAUNCH();
   return out;
 }

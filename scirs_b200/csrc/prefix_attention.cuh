@@ -27,8 +27,7 @@ struct Params {
   int T, rt_t;          // tails: splits (slots P .. P + T - 1), row tiles of a sequence
   // prefix on tcgen05: row tiles of tc_rows rows of one cached head against tc_blocks key blocks; a CTA takes
   // tc_share consecutive blocks of all row tiles' blocks laid end to end
-  int tc_rows, tc_tiles, tc_blocks, tc_streams;
-  long tc_share;
+  int tc_rows, tc_tiles, tc_blocks, tc_streams, tc_box, tc_share;
   float scale_log2;
   DevStatus* st;
 };

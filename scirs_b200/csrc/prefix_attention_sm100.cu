@@ -4,8 +4,10 @@
 // 512 threads, one CTA per SM:
 //   warp 0        issues the MMAs (one thread) and owns TMEM
 //   warps 4-7     producers: K and V blocks go through a ring of slots; unit 2 j is K of block j, 2 j + 1
-//                 its V, and unit u belongs to warp 4 + u % 4, which copies it with cp.async (16 bytes a
-//                 lane, any page size, written in the 128-byte swizzle that the MMA reads), waits for its
+//                 its V, and unit u belongs to warp 4 + u % 4. Where head_dim is 64 or 128 and the page size
+//                 a multiple of 8, whole blocks come by TMA, one box per run of tc_box slots of a page (a
+//                 lane each); the block that the prefix ends in, and everything else, by cp.async (16 bytes a
+//                 lane, zeros past the end, written in the same 128-byte swizzle): the warp waits for its
 //                 own copies, makes them visible to the asynchronous proxy and signals the slot full
 //   warps 8-15    two softmax warpgroups, a thread per row: read the row's 128 scores from TMEM, raise the
 //                 running maximum only when it grew by more than 2^8 (then O is rescaled in TMEM), write P
@@ -43,11 +45,50 @@ struct Tc {
   static constexpr int NS = HDP == 64 ? 8 : 4;  // ring slots
   static constexpr int OFF_Q = 0;               // two tiles
   static constexpr int OFF_RING = 2 * TILE;
-  static constexpr int OFF_BAR = OFF_RING + NS * TILE;
+  static constexpr int OFF_STAGE = OFF_RING + NS * TILE;  // 4 KB for each softmax warp's output
+  static constexpr int OFF_BAR = OFF_STAGE + 8 * 4096;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static constexpr uint32_t IDESC_S = umma_idesc_bf16(kBlk, kBlk, 0, 0);
   static constexpr uint32_t IDESC_O = umma_idesc_bf16(kBlk, HDP, 0, 1);
 };
+
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+// The MMAs are issued by a whole warp in uniform control flow with one lane predicated on: the compiler
+// then keeps the descriptors in uniform registers instead of moving them there for every instruction.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(on)
+      : "memory");
+}
 
 // A CTA's part of a row tile: blocks [j0, j0 + n).
 struct TcItem {
@@ -55,20 +96,22 @@ struct TcItem {
 };
 
 template <int STREAMS>
-__device__ __forceinline__ TcItem tc_item(const Params& p, long u, long end) {
+__device__ __forceinline__ TcItem tc_item(const Params& p, int u, int end) {
   TcItem i;
-  const long g = u / p.tc_blocks;
-  i.hk = (int)(g / p.tc_tiles);
-  i.r0 = (int)(g % p.tc_tiles) * p.tc_rows;
-  i.j0 = (int)(u % p.tc_blocks);
-  i.n = (int)min((long)(p.tc_blocks - i.j0), end - u);
-  i.slot = (int)(blockIdx.x - g * p.tc_blocks / p.tc_share) * STREAMS;
+  const int g = u / p.tc_blocks;
+  i.hk = g / p.tc_tiles;
+  i.r0 = (g - i.hk * p.tc_tiles) * p.tc_rows;
+  i.j0 = u - g * p.tc_blocks;
+  i.n = min(p.tc_blocks - i.j0, end - u);
+  i.slot = ((int)blockIdx.x - g * p.tc_blocks / p.tc_share) * STREAMS;
   i.tiles = STREAMS == 2 ? min(2, i.n) : (i.r0 + kBlk < p.B * p.Q * p.G ? 2 : 1);
   return i;
 }
 
 template <int HDP, int STREAMS>
-__global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p) {
+__global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_v,
+                                                                     const Params p) {
   using C = Tc<HDP>;
   constexpr int NS = C::NS;
   extern __shared__ uint8_t smem_raw[];
@@ -84,10 +127,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int chunks = p.HD / 8;  // 16-byte chunks of a row; the rest of a padded row stays zero
-  const long u_begin = blockIdx.x * p.tc_share;
-  const long u_end = min(u_begin + p.tc_share, (long)p.Hkv * p.tc_tiles * p.tc_blocks);
+  const int u_begin = blockIdx.x * p.tc_share;
+  const int u_end = min(u_begin + p.tc_share, p.Hkv * p.tc_tiles * p.tc_blocks);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -110,7 +153,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
     tmem_relinquish();
   }
   if (chunks < HDP / 8) {
-    for (int i = threadIdx.x; i < C::OFF_BAR / 16; i += kTcThreads)
+    for (int i = threadIdx.x; i < C::OFF_STAGE / 16; i += kTcThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
@@ -121,7 +164,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
 
   if (warp < 4) {
     setmaxnreg_dec<kRegsMma>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
+      const uint32_t on = elect_one_sync() ? 1u : 0u;
       // -------------------------------------------------------------- MMA
       const uint32_t q_addr = smem_u32(smem + C::OFF_Q), ring = smem_u32(smem + C::OFF_RING);
       int blk = 0;           // blocks of earlier items: unit 2 (blk + j) is K of block j
@@ -138,22 +182,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
 #pragma unroll
         for (int kk = 0; kk < HDP / 16; ++kk) {
           const uint32_t off = (kk >> 2) * (kBlk * 128) + (kk & 3) * 32;
-          tc_mma_f16_ss(tmem + t * kBlk, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
-                        C::IDESC_S, kk > 0 ? 1u : 0u);
+          mma_ss(tmem + t * kBlk, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024),
+                        C::IDESC_S, kk > 0 ? 1u : 0u, on);
         }
-        tc_commit(&s_full[t]);
+        mma_commit(&s_full[t], on);
       };
       auto issue_pv = [&](int t, int j, bool first) {
         const uint32_t va = ring + ((2 * (blk + j) + 1) % NS) * C::TILE;
 #pragma unroll
         for (int kk = 0; kk < kBlk / 16; ++kk)
           // A = P_t from TMEM (16 keys = 8 packed columns a step), B = V [keys][HDP] MN-major
-          tc_mma_f16_ts(tmem + 2 * kBlk + t * HDP, tmem + t * kBlk + kk * 8,
-                        umma_desc_sw128(va + kk * 2048, kBlk * 128, 1024), C::IDESC_O, !first || kk > 0 ? 1u : 0u);
+          mma_ts(tmem + 2 * kBlk + t * HDP, tmem + t * kBlk + kk * 8,
+                        umma_desc_sw128(va + kk * 2048, kBlk * 128, 1024), C::IDESC_O, !first || kk > 0 ? 1u : 0u, on);
       };
-      auto release = [&](int u) { tc_commit(&empty[u % NS]); };
+      auto release = [&](int u) { mma_commit(&empty[u % NS], on); };
       int ii = 0;
-      for (long u = u_begin; u < u_end && ok; ++ii) {
+      for (int u = u_begin; u < u_end && ok; ++ii) {
         const TcItem I = tc_item<STREAMS>(p, u, u_end);
         if (!mbar_wait(q_full, ii & 1, p.st, 101, abort_flag)) break;
         tc_fence_after();
@@ -162,7 +206,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
           if (!ok) break;
           for (int t = 0; t < I.tiles; ++t) issue_s(t, 0);
           release(2 * blk);
-          if (I.n == 1) tc_commit(q_empty);
+          if (I.n == 1) mma_commit(q_empty, on);
           for (int j = 0; j < I.n && ok; ++j) {
             for (int t = 0; t < I.tiles; ++t) {
               ok = ok && mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag);
@@ -176,13 +220,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
                 if (!ok) break;
                 issue_s(t, j + 1);
               } else {
-                tc_commit(&o_full[t]);
+                mma_commit(&o_full[t], on);
               }
             }
             if (!ok) break;
             release(2 * (blk + j) + 1);
             if (j + 1 < I.n) release(2 * (blk + j + 1));
-            if (j == I.n - 2) tc_commit(q_empty);
+            if (j == I.n - 2) mma_commit(q_empty, on);
           }
         } else {
           for (int t = 0; t < I.tiles && ok; ++t) {
@@ -191,7 +235,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
             issue_s(t, t);
             release(2 * (blk + t));
           }
-          if (ok && I.n <= 2) tc_commit(q_empty);
+          if (ok && I.n <= 2) mma_commit(q_empty, on);
           for (int j = 0; j < I.n && ok; ++j) {
             const int t = j & 1;
             ok = mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag) && wait_unit(2 * (blk + j) + 1);
@@ -205,22 +249,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
               if (!ok) break;
               issue_s(t, j + 2);
               release(2 * (blk + j + 2));
-              if (j + 3 == I.n) tc_commit(q_empty);
+              if (j + 3 == I.n) mma_commit(q_empty, on);
             } else {
-              tc_commit(&o_full[t]);
+              mma_commit(&o_full[t], on);
             }
           }
         }
         blk += I.n;
         u += I.n;
       }
-      tc_commit(drain);
+      mma_commit(drain, on);
       mbar_wait(drain, 0, nullptr, 0, nullptr);
     }
   } else if (warp < 8) {
     setmaxnreg_dec<kRegsLoad>();
     // ---------------------------------------------------------------- producers
     const int w = warp - 4;
+    const int box = p.tc_box;  // keys of a TMA box (0: cp.async only)
     constexpr int CPR = HDP / 8, RPI = 32 / CPR;  // chunks of a row, rows an instruction
     const int c = lane % CPR;
     const bf16* src = (w & 1) ? p.v : p.k;
@@ -228,16 +273,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
     const int max_pages = (p.L + p.bs - 1) / p.bs;
     int blk = 0;
     bool ok = true;
-    for (long u = u_begin; u < u_end && ok;) {
+    for (int u = u_begin; u < u_end && ok;) {
       const TcItem I = tc_item<STREAMS>(p, u, u_end);
       for (int j = 0; j < I.n; ++j) {
         const int unit = 2 * (blk + j) + (w & 1);
         if ((unit & 3) != w) continue;
+        const int key0 = (I.j0 + j) * kBlk;
+        if (box > 0 && key0 + kBlk <= p.L) {
+          const int key = key0 + lane * box;
+          int page = 0;
+          if (lane * box < kBlk) {
+            page = p.pages[key / p.bs];
+            if (!input_in_range(page, p.num_pages, p.st, 96)) page = 0;  // (reported: what is read in its place is void)
+          }
+          if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint64_t* bar = &full[unit % NS];
+          if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+          __syncwarp();
+          if (lane * box < kBlk) {
+            uint8_t* dst = smem + C::OFF_RING + (unit % NS) * C::TILE + lane * box * 128;
+#pragma unroll
+            for (int h = 0; h < HDP / 64; ++h)
+              tma_load_5d(dst + h * (kBlk * 128), (w & 1) ? &map_v : &map_k, bar, 0, key % p.bs, h, I.hk, page);
+          }
+          continue;
+        }
         // this lane looks four keys' rows up
         long row[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = (I.j0 + j) * kBlk + i * 32 + lane;
+          const int key = key0 + i * 32 + lane;
           row[i] = key < p.L ? pool_row(p, p.pages, max_pages, key, I.hk) : -1;
         }
         if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
@@ -274,18 +342,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
     const int slots = p.P + p.T;
     int cnt = 0, fin = 0, ii = 0;  // phases of s_full and o_full
     bool ok = true;
-    for (long u = u_begin; u < u_end && ok; ++ii) {
+    for (int u = u_begin; u < u_end && ok; ++ii) {
       const TcItem I = tc_item<STREAMS>(p, u, u_end);
       const int gr = I.r0 + (STREAMS == 2 ? 0 : t * kBlk) + r;
       const bf16* q = prefix_query(p, gr, I.hk);
       if (STREAMS == 1 || t == 0) {
         // Q of this row (zeros for a row that takes no part)
         if (!mbar_wait(q_empty, (ii & 1) ^ 1, p.st, 104, abort_flag)) break;
-        uint8_t* dst = smem + C::OFF_Q + t * C::TILE + r * 128;
-#pragma unroll 4
-        for (int c = 0; c < chunks; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kBlk * 128) + (((c ^ r) & 7) << 4)) =
-              q != nullptr ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
+        // the warp's 32 rows, a whole row (or two, four) per instruction; all loads before the first store
+        constexpr int CPR = HDP / 8, RPI = 32 / CPR;
+        const int c = lane % CPR;
+        uint4 x[32 / RPI];
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(q), i * RPI + lane / CPR);
+          x[i] = src != 0 && c < chunks ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+        }
+        uint8_t* dst = smem + C::OFF_Q + t * C::TILE + (warp & 3) * 32 * 128 + (c >> 3) * (kBlk * 128);
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int row = i * RPI + lane / CPR;
+          *reinterpret_cast<uint4*>(dst + row * 128 + (((c ^ row) & 7) << 4)) = x[i];
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -372,16 +450,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const Params p
         if (!mbar_wait(&o_full[t], fin & 1, p.st, 106, abort_flag)) break;
         ++fin;
         tc_fence_after();
+        // 32 columns at a time through shared memory, so that a store writes four rows' whole lines
+        uint8_t* stage = smem + C::OFF_STAGE + (warp - 8) * 4096;
+        long to[8];  // the rows that this lane stores, four lanes' rows apart
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          to[i] = __shfl_sync(0xffffffffu, live ? at * p.HD : -1L, i * 4 + (lane >> 3));
 #pragma unroll 1
         for (int c = 0; c < HDP; c += 32) {
           uint32_t ov[32];
           tmem_ld_32x32b_x32(o_base + c, ov);
           tc_wait_ld();
-          if (live) {
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c + e < p.HD)
-                *reinterpret_cast<uint4*>(p.part_o + at * p.HD + c + e) = make_uint4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ lane) & 7) * 16) =
+                make_uint4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3), e = lane & 7;
+            if (to[i] >= 0 && c + 4 * e < p.HD)
+              *reinterpret_cast<uint4*>(p.part_o + to[i] + c + 4 * e) =
+                  *reinterpret_cast<const uint4*>(stage + row * 128 + ((e ^ row) & 7) * 16);
           }
         }
         tc_fence_before();
@@ -408,17 +499,35 @@ void plan_prefix_tc(Params& p, int sms) {
   p.tc_rows = rows > kBlk ? 2 * kBlk : kBlk;
   p.tc_tiles = (rows + p.tc_rows - 1) / p.tc_rows;
   p.tc_blocks = (p.L + kBlk - 1) / kBlk;
-  const long units = (long)p.Hkv * p.tc_tiles * p.tc_blocks;
-  p.tc_share = std::max<long>(2, (units + sms - 1) / sms);
+  const int64_t units = (int64_t)p.Hkv * p.tc_tiles * p.tc_blocks;
+  TORCH_CHECK(units < (1LL << 30), "paged attention: too large");
+  p.tc_share = (int)std::max<int64_t>(2, (units + sms - 1) / sms);
   p.P = (int)((p.tc_blocks - 1) / p.tc_share + 2) * p.tc_streams;
+  // boxes of the largest power of two that divides the page size: at least the 8 rows of the swizzle
+  const int box = std::min(p.bs & -p.bs, kBlk);
+  p.tc_box = (p.HD == 64 || p.HD == 128) && box >= 8 ? box : 0;
+}
+
+// The pool as [page][head][64-column half][slot][64]: a box is tc_box slots of one half.
+static CUtensorMap pool_map(const Params& p, const bf16* pool) {
+  const uint64_t row = (uint64_t)p.Hkv * p.HD * 2;
+  const uint64_t ext[5] = {64, (uint64_t)p.bs, (uint64_t)p.HD / 64, (uint64_t)p.Hkv, (uint64_t)p.num_pages};
+  const uint64_t str[4] = {row, 128, (uint64_t)p.HD * 2, row * p.bs};
+  const uint32_t bx[5] = {64, (uint32_t)p.tc_box, 1, 1, 1};
+  return make_tmap_bf16(pool, 5, ext, str, bx, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int HDP, int STREAMS>
 static void launch_tc(const Params& p, cudaStream_t st) {
   auto kern = prefix_tc_kernel<HDP, STREAMS>;
   set_max_smem((const void*)kern, Tc<HDP>::SMEM);
-  const long units = (long)p.Hkv * p.tc_tiles * p.tc_blocks;
-  kern<<<(unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st>>>(p);
+  const int units = p.Hkv * p.tc_tiles * p.tc_blocks;
+  CUtensorMap mk{}, mv{};
+  if (p.tc_box > 0) {
+    mk = pool_map(p, p.k);
+    mv = pool_map(p, p.v);
+  }
+  kern<<<(unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st>>>(mk, mv, p);
 }
 
 void launch_prefix_tc(const Params& p, cudaStream_t st) {
