@@ -9,9 +9,9 @@ namespace prefix {
 
 using bf16 = __nv_bfloat16;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kTile = 16;  // keys per step of a warp
+constexpr int kTile = 16;  // keys per step of a warp: split lengths are multiples
 constexpr int kStages = 3;
-constexpr int kStep = kTile * kWarps;  // keys per step of a CTA: split lengths are multiples
+constexpr float kRaise = 8.f;  // a running maximum is raised only past 2^8
 
 struct Params {
   const bf16 *q, *k, *v;
@@ -22,9 +22,15 @@ struct Params {
   int table_stride, max_pages, num_pages;
   int B, Q, H, Hkv, G, HD, bs;
   int L;                // tokens of the prefix
-  int P;                // slots of a row that the prefix may take
-  int per_p, rt_p;      // prefix items of item_kernel: keys a split, row tiles (0: tcgen05 takes the prefix)
-  int T, rt_t;          // tails: splits (slots P .. P + T - 1), row tiles of a sequence
+  int P, T;             // slots of a row that the prefix and its tail may take: 0 .. P - 1, P .. P + T - 1
+  int rt_p, rt_t;       // item_kernel: row tiles of the prefix (0: tcgen05 takes it) and of a sequence
+  int item_rows;        // 16 MT
+  int pages_max;        // pages of the prefix
+  int share_min;        // fewest tiles of a warp's share
+  int box;              // keys of a TMA box (0: cp.async)
+  int* counts;          // [Hkv rt_p + B Hkv rt_t]: slots that item_kernel filled
+  uint32_t bs_mul;      // division by bs (see page_of)
+  int bs_shift;
   // prefix on tcgen05: row tiles of tc_rows rows of one cached head against tc_blocks key blocks; a CTA takes
   // tc_share consecutive blocks of all row tiles' blocks laid end to end
   int tc_rows, tc_tiles, tc_blocks, tc_streams, tc_box, tc_share;
@@ -36,32 +42,41 @@ struct Seq {
   int len, ql, start;  // tokens, queries, first key that is read through the sequence's own chain
 };
 
-__device__ __forceinline__ Seq seq_of(const Params& p, int b, bool report = false) {
+__device__ __forceinline__ Seq seq_from(const Params& p, int len, int ql, bool report) {
   Seq s;
-  s.len = max(p.lens[b], 0);
+  s.len = max(len, 0);
   if ((long)s.len > (long)p.max_pages * p.bs) {  // not addressable
     if (report) report_status(p.st, kStBounds, 95, (unsigned)s.len);
     s.len = p.max_pages * p.bs;
   }
-  s.ql = p.qlens != nullptr ? min(max(p.qlens[b], 0), p.Q) : p.Q;
+  s.ql = min(max(ql, 0), p.Q);
   if (s.ql == 0) s.len = 0;
   s.start = s.len - s.ql + 1 >= p.L ? p.L : 0;
   return s;
 }
 
-// Keys of a split of a sequence's tail: an even share, in whole steps.
-__device__ __forceinline__ int tail_share(const Params& p, const Seq& s) {
-  const int n = max(s.len - s.start, 0);
-  return ((n + p.T - 1) / p.T + kStep - 1) / kStep * kStep;
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+  return seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, false);
+}
+
+// The tiles of a sequence's tail begin at multiples of kTile; the first one may begin before the tail does.
+__device__ __forceinline__ int first_key(const Seq& s) { return s.start & ~(kTile - 1); }
+__device__ __forceinline__ int tail_tiles(const Seq& s) {
+  return s.len > s.start ? (s.len - first_key(s) + kTile - 1) / kTile : 0;
+}
+
+// key / bs for 0 <= key < 2^31: multiplication by the rounded-up reciprocal (Granlund & Montgomery, 1994).
+__device__ __forceinline__ int page_of(const Params& p, int key) {
+  return (int)(((uint64_t)(uint32_t)key * p.bs_mul) >> p.bs_shift);
 }
 
 // A K or V row (one token, one head) of the pool, in elements; -1 where the chain names no page of the pool.
 __device__ __forceinline__ long pool_row(const Params& p, const int* pages, int max_pages, int key, int hk) {
-  const int pi = key / p.bs;
+  const int pi = page_of(p, key);
   if (pi >= max_pages) return -1;
   const int page = pages[pi];
   if (!input_in_range(page, p.num_pages, p.st, 96)) return -1;
-  return (((long)page * p.bs + key % p.bs) * p.Hkv + hk) * p.HD;
+  return (((long)page * p.bs + key - pi * p.bs) * p.Hkv + hk) * p.HD;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool full) {
@@ -82,6 +97,18 @@ __device__ __forceinline__ const bf16* prefix_query(const Params& p, int r, int 
   if (t >= s.ql || s.start != p.L) return nullptr;
   return p.q + b * p.q_sb + t * p.q_st + (long)(hk * p.G + r % p.G) * p.q_sh;
 }
+
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+
+// A tensor map of a pool with boxes of `rows` slots of `halves` 64-column halves of one head (head_dim 64 or 128).
+CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves);
 
 // The prefix on tcgen05: plans the split (p.P and the tc_ fields), launches.
 void plan_prefix_tc(Params& p, int sms);

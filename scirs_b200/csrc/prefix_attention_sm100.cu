@@ -37,7 +37,6 @@ constexpr int kBlk = 128;  // keys of a block, rows of a tile
 // warpgroups: MMA, producers, two of softmax; 512 x 128 registers at launch
 constexpr int kRegsMma = 48, kRegsLoad = 56, kRegsSoftmax = 200;
 static_assert(kRegsMma + kRegsLoad + 2 * kRegsSoftmax <= 4 * 128, "register split exceeds the launch");
-constexpr float kRaise = 8.f;  // raise the reference maximum only past 2^8
 
 template <int HDP>
 struct Tc {
@@ -51,15 +50,6 @@ struct Tc {
   static constexpr uint32_t IDESC_S = umma_idesc_bf16(kBlk, kBlk, 0, 0);
   static constexpr uint32_t IDESC_O = umma_idesc_bf16(kBlk, HDP, 0, 1);
 };
-
-__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3, int c4) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
-      "[%2];" ::"r"(smem_u32(smem_dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
 
 // The MMAs are issued by a whole warp in uniform control flow with one lane predicated on: the compiler
 // then keeps the descriptors in uniform registers instead of moving them there for every instruction.
@@ -281,9 +271,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         const int key0 = (I.j0 + j) * kBlk;
         if (box > 0 && key0 + kBlk <= p.L) {
           const int key = key0 + lane * box;
+          const int slot_in_page = key - page_of(p, key) * p.bs;
           int page = 0;
           if (lane * box < kBlk) {
-            page = p.pages[key / p.bs];
+            page = p.pages[page_of(p, key)];
             if (!input_in_range(page, p.num_pages, p.st, 96)) page = 0;  // (reported: what is read in its place is void)
           }
           if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
@@ -297,7 +288,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
             uint8_t* dst = smem + C::OFF_RING + (unit % NS) * C::TILE + lane * box * 128;
 #pragma unroll
             for (int h = 0; h < HDP / 64; ++h)
-              tma_load_5d(dst + h * (kBlk * 128), (w & 1) ? &map_v : &map_k, bar, 0, key % p.bs, h, I.hk, page);
+              tma_load_5d(dst + h * (kBlk * 128), (w & 1) ? &map_v : &map_k, bar, 0, slot_in_page, h, I.hk, page);
           }
           continue;
         }
@@ -508,15 +499,6 @@ void plan_prefix_tc(Params& p, int sms) {
   p.tc_box = (p.HD == 64 || p.HD == 128) && box >= 8 ? box : 0;
 }
 
-// The pool as [page][head][64-column half][slot][64]: a box is tc_box slots of one half.
-static CUtensorMap pool_map(const Params& p, const bf16* pool) {
-  const uint64_t row = (uint64_t)p.Hkv * p.HD * 2;
-  const uint64_t ext[5] = {64, (uint64_t)p.bs, (uint64_t)p.HD / 64, (uint64_t)p.Hkv, (uint64_t)p.num_pages};
-  const uint64_t str[4] = {row, 128, (uint64_t)p.HD * 2, row * p.bs};
-  const uint32_t bx[5] = {64, (uint32_t)p.tc_box, 1, 1, 1};
-  return make_tmap_bf16(pool, 5, ext, str, bx, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <int HDP, int STREAMS>
 static void launch_tc(const Params& p, cudaStream_t st) {
   auto kern = prefix_tc_kernel<HDP, STREAMS>;
@@ -524,8 +506,8 @@ static void launch_tc(const Params& p, cudaStream_t st) {
   const int units = p.Hkv * p.tc_tiles * p.tc_blocks;
   CUtensorMap mk{}, mv{};
   if (p.tc_box > 0) {
-    mk = pool_map(p, p.k);
-    mv = pool_map(p, p.v);
+    mk = pool_map(p, p.k, p.tc_box, 1);
+    mv = pool_map(p, p.v, p.tc_box, 1);
   }
   kern<<<(unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st>>>(mk, mv, p);
 }

@@ -97,6 +97,8 @@ class PagedAttentionForward:
             raise InferenceError("query shape does not match the configuration")
         if self.config.num_heads % c.num_heads or self.config.head_dim != c.head_dim:
             raise InferenceError("the pool's heads do not match the configuration")
+        if not 0.0 < self._scale() < float("inf"):
+            raise InferenceError("scale must be positive and finite")
         if prefix_len < 0 or prefix_len > min(prefix_pages.numel(), block_tables.shape[-1]) * c.block_size:
             raise InferenceError("prefix_len is longer than the prefix's pages or a chain")
         if q.is_cuda:
