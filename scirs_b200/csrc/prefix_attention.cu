@@ -15,12 +15,12 @@
 //   A sequence some of whose queries end inside the prefix (it is shorter, or padding) is read by itself
 //   from its first key, so that in a prefix item a row sees every key or none.
 //
-// An item belongs to one warp. It walks its keys 16 at a time, K and V rows of one head copied into a ring of
-// its own: by TMA, a lane per box, where head_dim is 64 or 128 and the page size a multiple of 8, else by
-// cp.async (16 bytes a lane, the same swizzle, free of bank conflicts for ldmatrix); S = Q K^T and
-// O += P V by mma.sync m16n8k16 with the running max and sum in registers. No two warps ever wait for one
-// another, and the copies run ahead over the end of an item into the next one, their page ids read a step
-// before they are needed. Bound by memory as long as few rows share a key.
+// An item belongs to a CTA of four warps. Each walks every fourth tile of 16 keys, K and V rows of one head
+// copied into a ring of its own: by TMA where head_dim is 64 or 128 and the page size a multiple of 8, else by
+// cp.async (16 bytes a lane, the same swizzle, free of bank conflicts for ldmatrix); S = Q K^T and O += P V by
+// mma.sync m16n8k16 with the running max and sum in registers. The warps meet once, at the end. What bounds
+// an item is the chain length -> page ids -> first tile (so page ids are read 32 boxes at a time, and before
+// the length where the split does not depend on it), and memory over many items.
 //
 // Masked places (keys past a row's limit, slots past the length or before the item's first key) get P = 0
 // by selection. Where a tile has any and one of its V values is infinite or NaN, P V is formed row by row
@@ -57,8 +57,13 @@ template <int HDP>
 struct Cfg {
   static constexpr int HALF = kTile * 128;           // 64 columns of a K or V tile
   static constexpr int KV = HALF * (HDP / 64);       // a K or V tile
-  static constexpr int WARP = kStages * 2 * KV;      // a warp's ring
-  static constexpr int SMEM = kWarps * WARP + 1024;
+  static constexpr int STAGES = 3;
+  static constexpr int WARP = STAGES * 2 * KV;       // a warp's ring
+  // joining the warps at the end reuses the rings: 16 MT rows of O and (max, sum) a warp
+  static constexpr int smem(int mt) {
+    const int merge = kWarps * 16 * mt * (HDP + 2) * 4;
+    return (kWarps * WARP > merge ? kWarps * WARP : merge) + 1024;
+  }
   // per SM, by registers and shared memory
   static constexpr int ctas(int mt) { return HDP == 64 && mt == 1 ? 3 : 2; }
 };
@@ -71,185 +76,133 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)((c >> 3) * Cfg<HDP>::HALF + r * 128 + ((c ^ r) & 7) * 16);
 }
 
-// What a warp works on: a run of tiles of one segment, that is of 16 MT rows of one cached head against the
-// keys of the prefix or of a sequence's tail.
-struct Item {
-  bool is_prefix;
-  int hk, r0, r_end, seg;  // seg: index into counts
-  int b;                   // the sequence of a tail item
-  int key0, k0, k1;        // tiles from key0; keys [k0, k1)
-  int slot;
-  bool ends;               // the segment's last tile is the item's
-};
-
 template <int HDP, int MT, bool TMA>
 __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
                                                                              const Params p) {
   using C = Cfg<HDP>;
+  constexpr int M = 16 * MT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Item queue_s[kWarps][4];  // items on their way
-  __shared__ uint64_t full_s[kWarps][kStages];
+  __shared__ uint64_t full_s[kWarps][C::STAGES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* full = full_s[warp];
+  uint8_t* ring = smem + warp * C::WARP;
+  const uint32_t ring_a = smem_u32(ring);
+
+  // ---- which rows against which keys. Neighbouring items are the cached heads of the same keys, which lie
+  // side by side in a page.
+  int i = blockIdx.x;
+  const int hk = i % p.Hkv;
+  i /= p.Hkv;
+  const bool is_prefix = i < p.P * p.rt_p;  // (rt_p = 0 when tcgen05 takes the prefix)
+  int r0, r_end, split, b = 0;
+  const int* pages;
+  if (is_prefix) {
+    split = i % p.P;
+    r0 = i / p.P * M;
+    r_end = p.B * p.Q * p.G;
+    pages = p.pages;
+  } else {
+    i -= p.P * p.rt_p;
+    split = i % p.T;
+    i /= p.T;
+    b = i / p.rt_t;
+    r0 = b * p.Q * p.G + (i - b * p.rt_t) * M;
+    r_end = (b + 1) * p.Q * p.G;
+    pages = p.tables + (long)b * p.table_stride;
+  }
+  const int max_pages = is_prefix ? p.pages_max : p.max_pages;
+
+  // ---- page ids: with TMA a lane holds the page and slot of one box, 32 boxes of this warp's tiles at a time
+  // (tile j of the warp begins at base + (4 j + warp) 16); with cp.async lanes 0-15 hold one tile's keys
+  const int runs = TMA ? kTile / p.box : 1;  // boxes of a tile
+  int base = is_prefix ? split * p.per_p : p.L & ~(kTile - 1), k1 = 0x7fffffff;
+  int page = -2, at = 0, batch = 0;
+  auto look_up = [&](int j) {  // TMA: the boxes of tiles j, j + 1, ..; cp.async: the keys of tile j
+    const int key = TMA ? base + (((j + lane / runs) * kWarps + warp) * kTile + lane % runs * p.box)
+                        : base + (j * kWarps + warp) * kTile + lane;
+    const int pi = page_of(p, key);
+    page = (TMA || lane < kTile) && key >= 0 && key < k1 && pi < max_pages ? pages[pi] : -2;
+    at = key - pi * p.bs;
+    batch = j;
+  };
+  // the whole tail in one item: its pages can be read before its length is known
+  const bool early = TMA && (is_prefix || p.T == 1);
+  if (early) look_up(0);
+
+  int k0, len = 0, ql = 0;
+  if (is_prefix) {
+    k0 = base;
+    k1 = min(base + p.per_p, p.L);
+  } else {
+    const Seq s = seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, threadIdx.x == 0);
+    const int share = tail_share(p, s);
+    const int first = first_key(s) + split * share;
+    k0 = max(first, s.start);
+    k1 = min(first + share, s.len);
+    if (k0 >= k1) return;  // the combine kernel knows the splits that hold keys
+    len = s.len;
+    ql = s.ql;
+    if (first != base || !early) {
+      base = first;
+      if (TMA) look_up(0);
+    }
+  }
+  const int tiles = max((k1 - base + kTile - 1) / kTile - warp + kWarps - 1, 0) / kWarps;  // of this warp
   if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  __syncwarp();
-  uint8_t* ring = smem + warp * C::WARP;
-  const uint32_t ring_a = smem_u32(ring);
-  Item* queue = queue_s[warp];
   const int chunks = p.HD / 8;  // 16-byte chunks that a row has; the rest of a padded row stays zero
-  if (!TMA && chunks < HDP / 8) {
+  if (!TMA && chunks < HDP / 8)
     for (int j = lane; j < C::WARP / 16; j += 32) reinterpret_cast<uint4*>(ring)[j] = make_uint4(0, 0, 0, 0);
-    __syncwarp();
-  }
+  __syncwarp();
 
-  // ---- this warp's share of all tiles, laid end to end: the prefix's segments, then each sequence's
-  const int nseg_p = p.Hkv * p.rt_p, per_b = p.Hkv * p.rt_t;  // segments of the prefix, of a sequence
-  const int tiles_p = (p.L + kTile - 1) / kTile;
-  auto tiles_of = [&](int b) { return b < p.B ? tail_tiles(seq_of(p, b)) : 0; };
-  int total = 0, most = 0;
-#pragma unroll 4
-  for (int b = lane; b < p.B; b += 32) {
-    const int n = tiles_of(b);
-    total += n;
-    most = max(most, n);
-  }
-  total = nseg_p * tiles_p + __reduce_add_sync(0xffffffffu, total) * per_b;
-  most = __reduce_max_sync(0xffffffffu, most);
-  const int nw = gridDim.x * kWarps;
-  // (no tail may have more than T parts: sequences that end inside a long prefix can be longer than planned)
-  const int share = max(max(p.share_min, (total + nw - 1) / nw), (most + p.T - 3) / (p.T - 2));
-  // (few shares are spread over the SMs; of many, a CTA's warps take neighbours)
-  const int w = share * nw - total >= share * (nw / 2) ? warp * gridDim.x + blockIdx.x : blockIdx.x * kWarps + warp;
-  long u_at = (long)w * share;  // where the walk stands
-  const int u_end = (int)min(u_at + share, (long)total);
-
-  // ---- what is copied next; its page ids are read a step before they are used
-  int lk = 0, lk1 = 0, lhk = 0, lmax = 0, q_tail = 0;
-  const int* lpages = nullptr;
-  bool more = u_at < u_end;
-  // page and slot of key lk + lane * step for the lanes whose keys make up the tile (page -2: not read)
-  int page = -2, at = 0;
-  const int step = TMA ? p.box : 1;  // TMA: keys of a box; cp.async: single keys
-  auto look_up = [&]() {
-    const int key = lk + lane * step, pi = page_of(p, key);
-    page = lane * step < kTile && key < lk1 && pi < lmax ? lpages[pi] : -2;
-    at = key - pi * p.bs;
-  };
-  // the sequence that the walk is in, its first tile's place, and its tiles (from 32 read at a time)
-  int cb = -1, c_at = nseg_p * tiles_p, c_tiles = 0, c_seg = 0;
-  Seq cs{0, 0, 0};
-  auto next_item = [&]() {
-    if (u_at >= u_end) {
-      more = false;
-      return;
-    }
-    Item n;
-    int seg_at, seg_tiles;  // the segment's first tile's place, and its tiles
-    if (u_at < nseg_p * tiles_p) {
-      const int g = (int)u_at / tiles_p;
-      seg_at = g * tiles_p;
-      seg_tiles = tiles_p;
-      n.is_prefix = true;
-      n.hk = g / p.rt_p;
-      n.r0 = (g - n.hk * p.rt_p) * 16 * MT;
-      n.r_end = p.B * p.Q * p.G;
-      n.seg = g;
-      n.b = 0;
-      n.key0 = ((int)u_at - seg_at) * kTile;
-      n.k0 = n.key0;
-      lpages = p.pages;
-      lmax = p.pages_max;
-    } else {
-      while ((int)u_at >= c_at + c_tiles * per_b) {
-        c_at += c_tiles * per_b;
-        if (cb + 1 >= p.B) {  // (lengths that change under the kernel: nothing is read past the batch)
-          more = false;
-          return;
-        }
-        // on to the sequence that holds u_at, 32 at a time
-        const int b0 = cb + 1, mine = tiles_of(b0 + lane) * per_b;
-        int inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += x;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, c_at + inc > (int)u_at);
-        if (past == 0u) {
-          cb = b0 + 31;
-          c_at += __shfl_sync(0xffffffffu, inc, 31);
-          c_tiles = 0;
-        } else {
-          const int j = __ffs(past) - 1;
-          cb = b0 + j;
-          c_at += __shfl_sync(0xffffffffu, inc - mine, j);
-          cs = seq_of(p, cb);
-          c_tiles = tail_tiles(cs);
-          if (lane == 0 && p.lens[cb] > cs.len && cs.ql > 0) report_status(p.st, kStBounds, 95, (unsigned)p.lens[cb]);
-        }
-      }
-      const int g = ((int)u_at - c_at) / c_tiles;
-      seg_at = c_at + g * c_tiles;
-      seg_tiles = c_tiles;
-      n.is_prefix = false;
-      n.hk = g / p.rt_t;
-      n.b = cb;
-      n.r0 = cb * p.Q * p.G + (g - n.hk * p.rt_t) * 16 * MT;
-      n.r_end = (cb + 1) * p.Q * p.G;
-      n.seg = nseg_p + cb * per_b + g;
-      n.key0 = first_key(cs) + ((int)u_at - seg_at) * kTile;
-      n.k0 = max(n.key0, cs.start);
-      lpages = p.tables + (long)cb * p.table_stride;
-      lmax = p.max_pages;
-    }
-    const int n_tiles = min(seg_at + seg_tiles, u_end) - (int)u_at;
-    n.k1 = min(n.key0 + n_tiles * kTile, n.is_prefix ? p.L : cs.len);
-    n.slot = w - seg_at / share + (n.is_prefix ? 0 : p.P);
-    n.ends = (int)u_at + n_tiles == seg_at + seg_tiles;
-    u_at += n_tiles;
-    lk = n.key0;
-    lk1 = n.k1;
-    lhk = n.hk;
-    if (lane == 0) queue[q_tail & 3] = n;
-    ++q_tail;
-  };
-  // Copy the tile into a stage; returns which of its keys lie on pages of the pool (bit = key).
-  auto copy = [&](int stage) -> uint32_t {
+  // Copy tile j into a stage; returns which of its keys are to be used (bit = key).
+  auto copy = [&](int j, int stage) -> uint32_t {
     uint32_t valid;
-    const bool good = page != -2 && input_in_range(page, p.num_pages, p.st, 96);
-    const uint32_t ok = __ballot_sync(0xffffffffu, good);
     uint8_t* dst = ring + stage * 2 * C::KV;
+    const int key0 = base + (j * kWarps + warp) * kTile;
     if (TMA) {
-      // a lane per box: K or V of the whole tile, or of 8 keys and one half of the columns; a box that is
-      // not read is taken off the bytes to wait for
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], __popc(ok) * 2 * HDP * 2 * p.box);
-      __syncwarp();
-      if (p.box == kTile) {
-        const int pg = __shfl_sync(0xffffffffu, page, 0), slot = __shfl_sync(0xffffffffu, at, 0);
-        if (lane < 2 && ok != 0u)
-          tma_load_5d(dst + lane * C::KV, lane ? &map_v : &map_k, &full[stage], 0, slot, 0, lhk, pg);
-        valid = ok != 0u ? 0xffffu : 0u;
+      if ((j - batch + 1) * runs > 32) look_up(j);
+      // boxes of the whole tile, or, a lane each, of 8 keys and one half of the columns; a box that is not
+      // read is taken off the bytes to wait for
+      const int from = (j - batch) * runs;
+      const int pg0 = __shfl_sync(0xffffffffu, page, from), sl0 = __shfl_sync(0xffffffffu, at, from);
+      if (runs == 1) {
+        const bool good = pg0 != -2 && input_in_range(pg0, p.num_pages, p.st, 96);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[stage], good ? 2 * C::KV : 0);
+          if (good) {
+            tma_load_5d(dst, &map_k, &full[stage], 0, sl0, 0, hk, pg0);
+            tma_load_5d(dst + C::KV, &map_v, &full[stage], 0, sl0, 0, hk, pg0);
+          }
+        }
+        valid = good ? 0xffffu : 0u;
       } else {
-        const int i = lane & 1, h = lane >> 2;
-        const int pg = __shfl_sync(0xffffffffu, page, i), slot = __shfl_sync(0xffffffffu, at, i);
-        if (h < HDP / 64 && ((ok >> i) & 1u))
-          tma_load_5d(dst + (lane >> 1 & 1) * C::KV + h * C::HALF + i * 1024, (lane & 2) ? &map_v : &map_k,
-                      &full[stage], 0, slot, h, lhk, pg);
+        const int pg1 = __shfl_sync(0xffffffffu, page, from + 1), sl1 = __shfl_sync(0xffffffffu, at, from + 1);
+        // (ids that were read before the length may lie past the chain's end)
+        const int q = lane & 1, h = lane >> 2, pg = !q ? pg0 : key0 + 8 < k1 ? pg1 : -2;
+        const bool good = pg != -2 && input_in_range(pg, p.num_pages, p.st, 96);
+        const uint32_t ok = __ballot_sync(0xffffffffu, good) & 3u;
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], __popc(ok) * C::KV);
+        __syncwarp();
+        if (h < HDP / 64 && good)
+          tma_load_5d(dst + (lane >> 1 & 1) * C::KV + h * C::HALF + q * 1024, (lane & 2) ? &map_v : &map_k,
+                      &full[stage], 0, q ? sl1 : sl0, h, hk, pg);
         valid = (ok & 1u ? 0xffu : 0u) | (ok & 2u ? 0xff00u : 0u);
       }
     } else {
-      const long off = good ? (((long)page * p.bs + at) * p.Hkv + lhk) * p.HD : -1;
+      if (batch != j || j == 0) look_up(j);
+      const bool good = page != -2 && input_in_range(page, p.num_pages, p.st, 96);
+      const long off = good ? (((long)page * p.bs + at) * p.Hkv + hk) * p.HD : -1;
       constexpr int RPI = 32 / (HDP / 8);  // rows per instruction
       const int c = lane % (HDP / 8);
 #pragma unroll
-      for (int j = 0; j < kTile / RPI; ++j) {
-        const int r = j * RPI + lane / (HDP / 8);
+      for (int n = 0; n < kTile / RPI; ++n) {
+        const int r = n * RPI + lane / (HDP / 8);
         const long ro = __shfl_sync(0xffffffffu, off, r);
         if (c < chunks) {
           const uint32_t d = smem_u32(dst) + tile_at<HDP>(r, c);
@@ -259,79 +212,70 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
         }
       }
       cp_commit();
-      valid = ok;
+      valid = __ballot_sync(0xffffffffu, good);
+      look_up(j + 1);  // (in time for the next tile)
     }
+    if (key0 < k0) valid &= 0xffffu << (k0 - key0);
+    if (key0 + kTile > k1) valid &= 0xffffu >> (key0 + kTile - k1);
     return valid;
   };
 
-  // ---- the item that is worked on
-  Item it;
-  int q_head = 0, key0 = 0, lo = 0;
   int limit[MT][2];  // keys that rows r0 + 16 mt + lane / 4 (+ 8) see
   uint32_t qf[MT][HDP / 16][4];
   float o[MT][HDP / 8][4];
   float m_run[MT][2], l_run[MT][2];
-  // The queue's next item and its queries.
-  auto begin = [&]() {
-    __syncwarp();
-    it = queue[q_head & 3];
-    ++q_head;
-    key0 = it.key0;
-    Seq s{0, 0, 0};
-    if (!it.is_prefix) s = seq_of(p, it.b);
-    lo = 0x7fffffff;  // the smallest limit of a row that sees any of these keys
+  int lo = 0x7fffffff;  // the smallest limit of a row that sees any of these keys
+  int flying = 0, next = 0, s = 0, sw = 0;  // tiles on their way, the next one to copy; stages to read and to write
+  uint32_t phase = 0;
+  uint64_t valid_q = 0;  // 16 bits a tile on its way
+  for (int j = 0; j < tiles;) {
+    // (every piece of code stands in the loop once: what is fetched for the first time costs a short call most)
+    while (next < tiles && flying < C::STAGES) {
+      valid_q |= (uint64_t)copy(next, sw) << (16 * flying);
+      ++next;
+      ++flying;
+      sw = sw + 1 == C::STAGES ? 0 : sw + 1;
+    }
+    if (j == 0) {  // the queries, while the first tiles are on their way
+      const bf16* src[MT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = it.r0 + 16 * mt + 8 * h + (lane >> 2);
-        const int bt = r / p.G, b = bt / p.Q, t = bt - b * p.Q;
-        const bf16* src = p.q + b * p.q_sb + t * p.q_st + (long)(it.hk * p.G + r - bt * p.G) * p.q_sh;
+        for (int h = 0; h < 2; ++h) {
+          const int r = r0 + 16 * mt + 8 * h + (lane >> 2);
+          const int bt = r / p.G, rb = bt / p.Q, t = bt - rb * p.Q;
+          src[mt][h] = r < r_end ? p.q + rb * p.q_sb + t * p.q_st + (long)(hk * p.G + r - bt * p.G) * p.q_sh : nullptr;
+          int lim = 0;
+          if (r < r_end) {
+            if (is_prefix) {
+              const Seq q = seq_of(p, rb);
+              if (t < q.ql && q.start == p.L) lim = q.len - q.ql + t + 1;
+            } else if (t < ql) {
+              lim = max(len - ql + t + 1, 0);
+            }
+          }
+          limit[mt][h] = lim;
+          if (lim > k0) lo = min(lo, lim);
+          m_run[mt][h] = -INFINITY;
+          l_run[mt][h] = 0.f;
+#pragma unroll
+          for (int n = 0; n < HDP / 8; ++n) o[mt][n][2 * h] = o[mt][n][2 * h + 1] = 0.f;
+        }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int kk = 0; kk < HDP / 16; ++kk)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = kk * 16 + e * 8 + (lane & 3) * 2;
-            qf[mt][kk][e * 2 + h] = r < it.r_end && d < p.HD ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          for (int e = 0; e < 4; ++e) {
+            const int d = kk * 16 + (e >> 1) * 8 + (lane & 3) * 2;
+            qf[mt][kk][e] = src[mt][e & 1] != nullptr && d < p.HD
+                                ? __ldg(reinterpret_cast<const uint32_t*>(src[mt][e & 1] + d))
+                                : 0u;
           }
-        int lim = 0;
-        if (r < it.r_end) {
-          if (it.is_prefix) s = seq_of(p, b);
-          if (t < s.ql && (!it.is_prefix || s.start == p.L)) lim = max(s.len - s.ql + t + 1, 0);
-        }
-        limit[mt][h] = lim;
-        if (lim > it.k0) lo = min(lo, lim);
-        m_run[mt][h] = -INFINITY;
-        l_run[mt][h] = 0.f;
-#pragma unroll
-        for (int d = 0; d < HDP / 8; ++d) o[mt][d][2 * h] = o[mt][d][2 * h + 1] = 0.f;
-      }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-  };
-
-  // Every piece of code stands in the loop once: instructions that are fetched for the first time cost a
-  // short call more than anything else here.
-  bool primed = false, fresh = true;
-  int flying = 0, s = 0, sw = 0;  // tiles on their way; stages to read and to write
-  uint32_t phase = 0;
-  uint64_t valid = 0;  // 16 bits a tile on its way
-  while (true) {
-    while (more && flying < kStages) {
-      if (primed) {
-        valid |= (uint64_t)copy(sw) << (16 * flying);
-        ++flying;
-        sw = sw + 1 == kStages ? 0 : sw + 1;
-        lk += kTile;
-      }
-      primed = true;
-      if (lk >= lk1) next_item();
-      if (more) look_up();
+      lo = __reduce_min_sync(0xffffffffu, lo);
     }
-    if (flying == 0) break;
-    if (fresh) begin();
-    fresh = false;
     if (TMA) {
-      if (!mbar_wait(&full[s], phase, p.st, 97, nullptr)) return;
+      if (!mbar_wait(&full[s], phase, p.st, 97, nullptr)) break;
     } else {
       if (flying > 2)
         cp_wait<2>();
@@ -341,12 +285,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
         cp_wait<0>();
     }
     __syncwarp();
-    // the tile's keys that belong to the item and were read
-    uint32_t vm = (uint32_t)valid & 0xffffu;
-    valid >>= 16;
+    const uint32_t vm = (uint32_t)valid_q & 0xffffu;  // the tile's keys that are used
+    const int key0 = base + (j * kWarps + warp) * kTile;
+    ++j;
+    valid_q >>= 16;
     --flying;
-    if (key0 < it.k0) vm &= 0xffffu << (it.k0 - key0);
-    if (key0 + kTile > it.k1) vm &= 0xffffu >> (key0 + kTile - it.k1);
     uint8_t* const vt = ring + s * 2 * C::KV + C::KV;
     const uint32_t ka = ring_a + s * 2 * C::KV, va = ka + C::KV;
 
@@ -384,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
             const int kl = (e >> 1) * 8 + (lane & 3) * 2 + (e & 1);
             if (!((vm >> kl) & 1u) || key0 + kl >= limit[mt][h]) x[e] = -INFINITY;
           }
-        } else if (limit[mt][h] <= it.k0) {
+        } else if (limit[mt][h] <= k0) {
           x[0] = x[1] = x[2] = x[3] = -INFINITY;  // a row that sees nothing here
         }
         float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
@@ -464,36 +407,60 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
           }
         }
     }
-    __syncwarp();  // the tile has been read before the next step's copies overwrite it
-    key0 += kTile;
-    if (++s == kStages) {
+    __syncwarp();  // the tile has been read before the next copies overwrite it
+    if (++s == C::STAGES) {
       s = 0;
       phase ^= 1;
     }
-    if (key0 < it.k1) continue;
+  }
 
-    // ---- this split's part of every row
-    const int slots = p.P + p.T;
-    if (it.ends && lane == 0) p.counts[it.seg] = it.slot - (it.is_prefix ? 0 : p.P) + 1;
+  // ---- join the warps (the rings are free now), write this split's part of every row
+  float* mo = reinterpret_cast<float*>(smem);  // [warp][M][HDP]
+  float* mml = mo + kWarps * M * HDP;          // [warp][M][2]
+  __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = it.r0 + 16 * mt + 8 * h + (lane >> 2);
-        float l = l_run[mt][h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (r >= it.r_end) continue;
-        const int bt = r / p.G;
-        const long part = ((long)bt * p.H + it.hk * p.G + r - bt * p.G) * slots + it.slot;
-        if ((lane & 3) == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m_run[mt][h], l);
+    for (int h = 0; h < 2; ++h) {
+      const int r = 16 * mt + 8 * h + (lane >> 2);
+      float l = tiles > 0 ? l_run[mt][h] : 0.f;
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if ((lane & 3) == 0)
+        *reinterpret_cast<float2*>(mml + (warp * M + r) * 2) = make_float2(tiles > 0 ? m_run[mt][h] : -INFINITY, l);
+      if (tiles > 0 && r0 + r < r_end) {
 #pragma unroll
         for (int n = 0; n < HDP / 8; ++n)
-          if (n < chunks)
-            *reinterpret_cast<float2*>(p.part_o + part * p.HD + n * 8 + (lane & 3) * 2) =
-                make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+          *reinterpret_cast<float2*>(mo + (warp * M + r) * HDP + ((n * 8 + (lane & 3) * 2) ^ ((r & 3) * 8))) =
+              make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
       }
-    fresh = true;
+    }
+  __syncthreads();
+  const int slots = p.P + p.T;
+  for (int r = warp; r < M && r0 + r < r_end; r += kWarps) {
+    float m = -INFINITY, f[kWarps], l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mml[(w * M + r) * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      f[w] = ex2_fast(mml[(w * M + r) * 2] - ref);
+      l += f[w] * mml[(w * M + r) * 2 + 1];
+    }
+    const int gr = r0 + r, bt = gr / p.G;
+    const long part = ((long)bt * p.H + hk * p.G + gr - bt * p.G) * slots + (is_prefix ? split : p.P + split);
+    for (int d = lane * 2; d < p.HD; d += 64) {
+      float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        if (f[w] != 0.f) {  // (a warp without keys holds nothing)
+          const float2 x = *reinterpret_cast<const float2*>(mo + (w * M + r) * HDP + (d ^ ((r & 3) * 8)));
+          acc.x += f[w] * x.x;
+          acc.y += f[w] * x.y;
+        }
+      *reinterpret_cast<float2*>(p.part_o + part * p.HD + d) = acc;
+    }
+    if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
   }
 }
 
@@ -508,35 +475,39 @@ CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves) {
 
 // One CTA per output row; its warps take every fourth part.
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
-  const long row = blockIdx.x;
+  const int row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ float4 acc_s[4][32];
   __shared__ float den_s[4];
-  const int b = (int)(row / ((long)p.Q * p.H));
-  const int t = (int)(row / p.H % p.Q);
+  const int bt = row / p.H, h = row - bt * p.H, b = bt / p.Q, t = bt - b * p.Q;
+  const int slots = p.P + p.T;
+  const float* ml = p.part_ml + (long)row * slots * 2;
+  const float* po = p.part_o + (long)row * slots * p.HD;
+  // a lane reads the maximum of one slot; it does not wait for the length that says whether the slot is used
+  float mine = lane < slots ? ml[2 * lane] : -INFINITY;
   const Seq s = seq_of(p, b);
   // the slots that hold parts of this row: the prefix's, if the sequence takes part in it, and its tail's
-  const int h = (int)(row % p.H), hk = h / p.G, r = (b * p.Q + t) * p.G + h % p.G;
   int np = 0, nt = 0;
-  if (t < s.ql && s.start == p.L && p.L > 0) {
-    if (p.tc_share > 0) {
-      // the CTAs whose blocks meet the row tile's
-      const int first = (hk * p.tc_tiles + r / p.tc_rows) * p.tc_blocks;
-      np = ((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
-    } else {
-      np = p.counts[hk * p.rt_p + r / p.item_rows];
+  if (t < s.ql) {
+    if (s.start == p.L) {
+      np = p.P;
+      if (p.tc_share > 0) {
+        // the CTAs whose blocks meet the row tile's
+        const int hk = h / p.G, r = bt * p.G + h - hk * p.G;
+        const int first = (hk * p.tc_tiles + r / p.tc_rows) * p.tc_blocks;
+        np = ((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
+      }
     }
+    const int n = tail_keys(s), share = tail_share(p, s);
+    if (n > 0) nt = (n + share - 1) / share;
   }
-  if (t < s.ql && s.len > s.start)
-    nt = p.counts[p.Hkv * p.rt_p + (b * p.Hkv + hk) * p.rt_t + (r - b * p.Q * p.G) / p.item_rows];
-  const int slots = p.P + p.T;
-  const float* ml = p.part_ml + row * slots * 2;
-  const float* po = p.part_o + row * slots * p.HD;
-  const auto slot_of = [&](int j) { return j < np ? j : p.P + j - np; };
-  float m = -INFINITY;
-  for (int j = lane; j < np + nt; j += 32) m = fmaxf(m, ml[2 * slot_of(j)]);
+  const auto used = [&](int i) { return i < np || (i >= p.P && i < p.P + nt); };
+  float m = used(lane) ? mine : -INFINITY;
+  for (int i = lane + 32; i < slots; i += 32)
+    if (used(i)) m = fmaxf(m, ml[2 * i]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
+  const auto slot_of = [&](int j) { return j < np ? j : p.P + j - np; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.f;
   const bool on = 4 * lane < p.HD;
@@ -572,7 +543,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
     const float inv = 1.f / den;
     out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   }
-  *reinterpret_cast<uint2*>(p.out + row * p.HD + 4 * lane) = out;
+  *reinterpret_cast<uint2*>(p.out + (long)row * p.HD + 4 * lane) = out;
 }
 
 }  // namespace prefix
@@ -581,7 +552,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 // Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
 constexpr int64_t kTcRows = 32, kTcKeys = 256;
-constexpr int64_t kMinTiles = 4;
+constexpr int64_t kMinKeys = 128;
 
 torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
                                      torch::Tensor lens, torch::Tensor pages, int64_t L,
@@ -656,22 +627,23 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   const int mt = std::max(L > 0 && !tc ? rows : 0, seq_rows) > 16 ? 2 : 1;
   p.rt_p = L > 0 && !tc ? (int)((rows + 16 * mt - 1) / (16 * mt)) : 0;
   p.rt_t = (int)((seq_rows + 16 * mt - 1) / (16 * mt));
-  p.item_rows = 16 * mt;
   p.pages_max = (int)((L + bs - 1) / bs);
   p.bs_shift = 31;
   while ((1LL << (p.bs_shift - 31)) < bs) ++p.bs_shift;
   p.bs_mul = (uint32_t)(((1ULL << p.bs_shift) + bs - 1) / bs);
-  // All tiles of 16 keys are cut into equal shares, one for each warp, by the lengths on the device. The
-  // smallest share bounds the parts of a row: an eighth of what a warp gets if every chain is full, at least
-  // kMinTiles.
-  const int64_t ctas = (int64_t)sms * (HD <= 64 ? prefix::Cfg<64>::ctas(mt) : prefix::Cfg<128>::ctas(mt));
-  const int64_t prefix_tiles = (L + prefix::kTile - 1) / prefix::kTile;
-  const int64_t span_tiles = (max_pages * bs - L) / prefix::kTile + 2, chain_tiles = max_pages * bs / prefix::kTile + 2;
-  const int64_t work = Hkv * (p.rt_p * prefix_tiles + B * p.rt_t * span_tiles);
-  TORCH_CHECK(Hkv * (p.rt_p * prefix_tiles + B * p.rt_t * chain_tiles) < (1LL << 30), "paged attention: too large");
-  p.share_min = (int)std::max<int64_t>(kMinTiles, work / (ctas * prefix::kWarps * 8));
-  p.P = p.rt_p > 0 ? (int)((prefix_tiles - 1) / p.share_min + 2) : 0;
-  p.T = (int)(span_tiles / p.share_min + 3);
+  // two rounds of CTAs, of at least kMinKeys keys each
+  const int64_t ctas = 2LL * sms * (HD <= 64 ? prefix::Cfg<64>::ctas(mt) : prefix::Cfg<128>::ctas(mt));
+  const int64_t span = max_pages * bs - L;
+  const auto splits = [&](int64_t tiles, int64_t keys) {
+    return std::max<int64_t>(1, std::min(ctas / std::max<int64_t>(1, Hkv * tiles), (keys + kMinKeys - 1) / kMinKeys));
+  };
+  p.P = 0;
+  if (p.rt_p > 0) {
+    const int64_t n = splits(p.rt_p, L);
+    p.per_p = (int)(((L + n - 1) / n + prefix::kTile - 1) / prefix::kTile * prefix::kTile);
+    p.P = (int)((L + p.per_p - 1) / p.per_p);
+  }
+  p.T = (int)splits(B * p.rt_t, span);
   // boxes of a power of two that divides the page size, at least the 8 rows of the swizzle
   const int run = p.bs & -p.bs;
   p.box = (HD == 64 || HD == 128) && run >= 8 ? std::min(run, prefix::kTile) : 0;
@@ -681,8 +653,8 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   auto part_ml = at::empty({B * Q * H, slots, 2}, q.options().dtype(at::kFloat));
   p.part_o = part_o.data_ptr<float>();
   p.part_ml = part_ml.data_ptr<float>();
-  auto counts = at::empty({Hkv * (p.rt_p + B * p.rt_t)}, lens.options());
-  p.counts = counts.data_ptr<int>();
+  const int64_t items = Hkv * ((int64_t)p.rt_p * p.P + B * p.rt_t * p.T);
+  TORCH_CHECK(items < (1LL << 31), "paged attention: too large");
   if (tc) {
     prefix::launch_prefix_tc(p, cur_stream());
     SCIRS_CHECK_LAUNCH();
@@ -693,11 +665,12 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
     map_k = prefix::pool_map(p, p.k, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
     map_v = prefix::pool_map(p, p.v, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
   }
-#define SCIRS_ITEMS(HDP_, MT_, TMA_)                                                                                   \
-  {                                                                                                                    \
-    auto kern = prefix::item_kernel<HDP_, MT_, TMA_>;                                                                  \
-    set_max_smem((const void*)kern, prefix::Cfg<HDP_>::SMEM);                                                          \
-    kern<<<(unsigned)std::min<int64_t>(work, ctas), prefix::kThreads, prefix::Cfg<HDP_>::SMEM, st>>>(map_k, map_v, p); \
+#define SCIRS_ITEMS(HDP_, MT_, TMA_)                                                                                \
+  {                                                                                                                 \
+    auto kern = prefix::item_kernel<HDP_, MT_, TMA_>;                                                               \
+    constexpr int smem = prefix::Cfg<HDP_>::smem(MT_);                                                              \
+    set_max_smem((const void*)kern, smem);                                                                          \
+    kern<<<(unsigned)items, prefix::kThreads, smem, st>>>(map_k, map_v, p);                                         \
   }
 #define SCIRS_ITEMS_MT(HDP_, TMA_) \
   if (mt == 1) SCIRS_ITEMS(HDP_, 1, TMA_) else SCIRS_ITEMS(HDP_, 2, TMA_)

@@ -10,7 +10,6 @@ namespace prefix {
 using bf16 = __nv_bfloat16;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 16;  // keys per step of a warp: split lengths are multiples
-constexpr int kStages = 3;
 constexpr float kRaise = 8.f;  // a running maximum is raised only past 2^8
 
 struct Params {
@@ -22,13 +21,10 @@ struct Params {
   int table_stride, max_pages, num_pages;
   int B, Q, H, Hkv, G, HD, bs;
   int L;                // tokens of the prefix
-  int P, T;             // slots of a row that the prefix and its tail may take: 0 .. P - 1, P .. P + T - 1
-  int rt_p, rt_t;       // item_kernel: row tiles of the prefix (0: tcgen05 takes it) and of a sequence
-  int item_rows;        // 16 MT
+  int P, T;             // splits of the prefix and of a tail, and their slots: 0 .. P - 1, P .. P + T - 1
+  int per_p, rt_p, rt_t;  // item_kernel: keys of a prefix split; row tiles of the prefix (0: tcgen05 takes it), of a tail
   int pages_max;        // pages of the prefix
-  int share_min;        // fewest tiles of a warp's share
   int box;              // keys of a TMA box (0: cp.async)
-  int* counts;          // [Hkv rt_p + B Hkv rt_t]: slots that item_kernel filled
   uint32_t bs_mul;      // division by bs (see page_of)
   int bs_shift;
   // prefix on tcgen05: row tiles of tc_rows rows of one cached head against tc_blocks key blocks; a CTA takes
@@ -59,10 +55,12 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   return seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, false);
 }
 
-// The tiles of a sequence's tail begin at multiples of kTile; the first one may begin before the tail does.
+// The tiles of a sequence's tail begin at multiples of kTile, the first one perhaps before the tail does; the
+// keys from there, and a split's share of them.
 __device__ __forceinline__ int first_key(const Seq& s) { return s.start & ~(kTile - 1); }
-__device__ __forceinline__ int tail_tiles(const Seq& s) {
-  return s.len > s.start ? (s.len - first_key(s) + kTile - 1) / kTile : 0;
+__device__ __forceinline__ int tail_keys(const Seq& s) { return s.len > s.start ? s.len - first_key(s) : 0; }
+__device__ __forceinline__ int tail_share(const Params& p, const Seq& s) {
+  return ((tail_keys(s) + p.T - 1) / p.T + kTile - 1) / kTile * kTile;
 }
 
 // key / bs for 0 <= key < 2^31: multiplication by the rounded-up reciprocal (Granlund & Montgomery, 1994).
