@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
                                                                              const Params p) {
   using C = Cfg<HDP>;
   constexpr int M = 16 * MT;
+  allow_next();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_s[kWarps][C::STAGES];
@@ -141,7 +142,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     const int first = first_key(s) + split * share;
     k0 = max(first, s.start);
     k1 = min(first + share, s.len);
-    if (k0 >= k1) return;  // the combine kernel knows the splits that hold keys
+    if (k0 >= k1) {  // the combine kernel knows the splits that hold keys
+      wait_for_previous();
+      return;
+    }
     len = s.len;
     ql = s.ql;
     if (first != base || !early) {
@@ -462,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     }
     if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
   }
+  wait_for_previous();
 }
 
 // The pool as [page][head][64-column half][slot][64]: a box is `rows` slots of `halves` halves.
@@ -483,9 +488,10 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const int slots = p.P + p.T;
   const float* ml = p.part_ml + (long)row * slots * 2;
   const float* po = p.part_o + (long)row * slots * p.HD;
-  // a lane reads the maximum of one slot; it does not wait for the length that says whether the slot is used
-  float mine = lane < slots ? ml[2 * lane] : -INFINITY;
   const Seq s = seq_of(p, b);
+  wait_for_previous();
+  // a lane reads the maximum of one slot
+  const float mine = lane < slots ? ml[2 * lane] : -INFINITY;
   // the slots that hold parts of this row: the prefix's, if the sequence takes part in it, and its tail's
   int np = 0, nt = 0;
   if (t < s.ql) {
@@ -657,7 +663,6 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   TORCH_CHECK(items < (1LL << 31), "paged attention: too large");
   if (tc) {
     prefix::launch_prefix_tc(p, cur_stream());
-    SCIRS_CHECK_LAUNCH();
   }
   auto st = cur_stream();
   CUtensorMap map_k{}, map_v{};
@@ -670,7 +675,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
     auto kern = prefix::item_kernel<HDP_, MT_, TMA_>;                                                               \
     constexpr int smem = prefix::Cfg<HDP_>::smem(MT_);                                                              \
     set_max_smem((const void*)kern, smem);                                                                          \
-    kern<<<(unsigned)items, prefix::kThreads, smem, st>>>(map_k, map_v, p);                                         \
+    prefix::launch(kern, (unsigned)items, prefix::kThreads, smem, st, tc, map_k, map_v, p);                         \
   }
 #define SCIRS_ITEMS_MT(HDP_, TMA_) \
   if (mt == 1) SCIRS_ITEMS(HDP_, 1, TMA_) else SCIRS_ITEMS(HDP_, 2, TMA_)
@@ -681,9 +686,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   }
 #undef SCIRS_ITEMS_MT
 #undef SCIRS_ITEMS
-  SCIRS_CHECK_LAUNCH();
-  prefix::combine_kernel<<<(unsigned)(B * Q * H), 128, 0, st>>>(p);
-  SCIRS_CHECK_LAUNCH();
+  prefix::launch(prefix::combine_kernel, (unsigned)(B * Q * H), 128, 0, st, true, p);
   return out;
 }
 

@@ -108,6 +108,28 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
 // A tensor map of a pool with boxes of `rows` slots of `halves` 64-column halves of one head (head_dim 64 or 128).
 CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves);
 
+// The kernels of one call overlap at their ends: each may start when the one before it has started all its
+// CTAs, and waits for its completion where it needs it. Every kernel waits before it ends, so that a kernel
+// behind it finds all of them done.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launch; `overlap`: may start before the kernel in front of it in the stream has ended.
+template <typename... P, typename... A>
+void launch(void (*kern)(P...), unsigned grid, int threads, int smem, cudaStream_t st, bool overlap, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  SCIRS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
+}
+
 // The prefix on tcgen05: plans the split (p.P and the tc_ fields), launches.
 void plan_prefix_tc(Params& p, int sms);
 void launch_prefix_tc(const Params& p, cudaStream_t st);

@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
+  allow_next();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int chunks = p.HD / 8;  // 16-byte chunks of a row; the rest of a padded row stays zero
   const int u_begin = blockIdx.x * p.tc_share;
@@ -509,7 +510,7 @@ static void launch_tc(const Params& p, cudaStream_t st) {
     mk = pool_map(p, p.k, p.tc_box, 1);
     mv = pool_map(p, p.v, p.tc_box, 1);
   }
-  kern<<<(unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st>>>(mk, mv, p);
+  launch(kern, (unsigned)((units + p.tc_share - 1) / p.tc_share), kTcThreads, Tc<HDP>::SMEM, st, false, mk, mv, p);
 }
 
 void launch_prefix_tc(const Params& p, cudaStream_t st) {
