@@ -334,9 +334,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
         } else if (limit[mt][h] <= k0) {
           x[0] = x[1] = x[2] = x[3] = -INFINITY;  // a row that sees nothing here
         }
-        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        float mx = max_nan(max_nan(x[0], x[1]), x[2], x[3]);
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         mx *= p.scale_log2;
         // the reference maximum is raised only when it grew by more than 2^8: P stays below 2^8
         alpha[mt][h] = 1.f;
@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
           m_run[mt][h] = mx;
           rescale = true;
         }
+        if (!(mx < INFINITY)) m_run[mt][h] = NAN;  // a score that is NaN or infinite makes the row NaN
         const float ref = m_run[mt][h] == -INFINITY ? 0.f : m_run[mt][h];
         float sum = 0.f;
 #pragma unroll
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
   for (int r = warp; r < M && r0 + r < r_end; r += kWarps) {
     float m = -INFINITY, f[kWarps], l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, mml[(w * M + r) * 2]);
+    for (int w = 0; w < kWarps; ++w) m = max_nan(m, mml[(w * M + r) * 2]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {

@@ -68,6 +68,18 @@ __device__ __forceinline__ int page_of(const Params& p, int key) {
   return (int)(((uint64_t)(uint32_t)key * p.bs_mul) >> p.bs_shift);
 }
 
+// The largest value, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A K or V row (one token, one head) of the pool, in elements; -1 where the chain names no page of the pool.
 __device__ __forceinline__ long pool_row(const Params& p, const int* pages, int max_pages, int key, int hk) {
   const int pi = page_of(p, key);

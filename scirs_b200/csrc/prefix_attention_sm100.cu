@@ -38,6 +38,27 @@ constexpr int kBlk = 128;  // keys of a block, rows of a tile
 constexpr int kRegsMma = 48, kRegsLoad = 56, kRegsSoftmax = 200;
 static_assert(kRegsMma + kRegsLoad + 2 * kRegsSoftmax <= 4 * 128, "register split exceeds the launch");
 
+constexpr int kPoly = 5, kPolyOf = 16;  // pairs of exponentials on the FMA pipe
+
+// 2^x of a pair on the FMA pipe: x = n + f with n the nearest integer (added into the low mantissa bits of
+// 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f by a cubic fitted to the relative error there (Remez, 7.5e-5: below
+// the bf16 rounding of P by a factor of 50); 2^n by an addition to the exponent field. x is at most
+// kRaise; below -125 the result stays at 2^-125.
+__device__ __forceinline__ void exp2_poly_pair(float& x0, float& x1) {
+  const uint64_t big = f2_pack(12582912.f, 12582912.f), nbig = f2_pack(-12582912.f, -12582912.f);
+  const uint64_t x = f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const uint64_t n = f2_add(x, big);
+  const uint64_t f = f2_fma(f2_add(n, nbig), f2_pack(-1.f, -1.f), x);
+  uint64_t q = f2_fma(f2_pack(5.517166906e-02f, 5.517166906e-02f), f, f2_pack(2.426111222e-01f, 2.426111222e-01f));
+  q = f2_fma(q, f, f2_pack(6.932609855e-01f, 6.932609855e-01f));
+  q = f2_fma(q, f, f2_pack(9.999280735e-01f, 9.999280735e-01f));
+  float q0, q1, n0, n1;
+  f2_unpack(q, q0, q1);
+  f2_unpack(n, n0, n1);
+  x0 = __int_as_float(__float_as_int(q0) + (__float_as_int(n0) << 23));
+  x1 = __int_as_float(__float_as_int(q1) + (__float_as_int(n1) << 23));
+}
+
 template <int HDP>
 struct Tc {
   static constexpr int TILE = kBlk * HDP * 2;  // a Q tile, or K or V of a block
@@ -109,8 +130,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [NS]
   uint64_t* empty = full + NS;                                      // [NS]
   uint64_t* s_full = empty + NS;                                    // [2]
-  uint64_t* p_full = s_full + 2;                                    // [2]
-  uint64_t* o_full = p_full + 2;                                    // [2]
+  uint64_t* p_full = s_full + 2;                                    // [2][2]: halves of P_t
+  uint64_t* o_full = p_full + 4;                                    // [2]
   uint64_t* q_full = o_full + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* drain = q_empty + 1;
@@ -130,7 +151,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[2 * t], 4);
+      mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(q_full, STREAMS == 2 ? 4 : 8);
@@ -178,13 +200,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         }
         mma_commit(&s_full[t], on);
       };
-      auto issue_pv = [&](int t, int j, bool first) {
+      auto issue_pv = [&](int t, int j, int half, bool first) {
         const uint32_t va = ring + ((2 * (blk + j) + 1) % NS) * C::TILE;
 #pragma unroll
-        for (int kk = 0; kk < kBlk / 16; ++kk)
+        for (int k2 = 0; k2 < kBlk / 32; ++k2) {
+          const int kk = half * (kBlk / 32) + k2;
           // A = P_t from TMEM (16 keys = 8 packed columns a step), B = V [keys][HDP] MN-major
           mma_ts(tmem + 2 * kBlk + t * HDP, tmem + t * kBlk + kk * 8,
-                        umma_desc_sw128(va + kk * 2048, kBlk * 128, 1024), C::IDESC_O, !first || kk > 0 ? 1u : 0u, on);
+                 umma_desc_sw128(va + kk * 2048, kBlk * 128, 1024), C::IDESC_O, !first || kk > 0 ? 1u : 0u, on);
+        }
+      };
+      // P_t V in two halves: the first runs while the softmax warps work on the second
+      auto pv = [&](int t, int j, bool first, bool wait_v) -> bool {
+        if (!mbar_wait(&p_full[2 * t], done[t] & 1, p.st, 102, abort_flag)) return false;
+        if (wait_v && !wait_unit(2 * (blk + j) + 1)) return false;
+        tc_fence_after();
+        issue_pv(t, j, 0, first);
+        if (!mbar_wait(&p_full[2 * t + 1], done[t] & 1, p.st, 102, abort_flag)) return false;
+        ++done[t];
+        tc_fence_after();
+        issue_pv(t, j, 1, first);
+        return true;
       };
       auto release = [&](int u) { mma_commit(&empty[u % NS], on); };
       int ii = 0;
@@ -200,12 +236,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           if (I.n == 1) mma_commit(q_empty, on);
           for (int j = 0; j < I.n && ok; ++j) {
             for (int t = 0; t < I.tiles; ++t) {
-              ok = ok && mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag);
-              if (ok && t == 0) ok = wait_unit(2 * (blk + j) + 1);
+              ok = pv(t, j, j == 0, t == 0);
               if (!ok) break;
-              ++done[t];
-              tc_fence_after();
-              issue_pv(t, j, j == 0);
               if (j + 1 < I.n) {
                 if (t == 0) ok = wait_unit(2 * (blk + j + 1));
                 if (!ok) break;
@@ -229,11 +261,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           if (ok && I.n <= 2) mma_commit(q_empty, on);
           for (int j = 0; j < I.n && ok; ++j) {
             const int t = j & 1;
-            ok = mbar_wait(&p_full[t], done[t] & 1, p.st, 102, abort_flag) && wait_unit(2 * (blk + j) + 1);
+            ok = pv(t, j, j < 2, true);
             if (!ok) break;
-            ++done[t];
-            tc_fence_after();
-            issue_pv(t, j, j < 2);
             release(2 * (blk + j) + 1);
             if (j + 2 < I.n) {
               ok = wait_unit(2 * (blk + j + 2));
@@ -368,26 +397,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           break;
         }
         tc_fence_after();
+        // the row's 128 scores; the maximum of one half is taken while the other comes
         float sv[kBlk];
-        {
-          uint32_t* x = reinterpret_cast<uint32_t*>(sv);
-#pragma unroll
-          for (int c = 0; c < kBlk; c += 32) tmem_ld_32x32b_x32(s_base + c, x + c);
-          tc_wait_ld();
-        }
+        uint32_t* x = reinterpret_cast<uint32_t*>(sv);
+        tmem_ld_32x32b_x32(s_base, x);
+        tmem_ld_32x32b_x32(s_base + 32, x + 32);
+        tc_wait_ld_regs(x);
+        tc_wait_ld_regs(x + 32);
+        tmem_ld_32x32b_x32(s_base + 64, x + 64);
+        tmem_ld_32x32b_x32(s_base + 96, x + 96);
         const int left = p.L - (I.j0 + (STREAMS == 2 ? 2 * j + t : j)) * kBlk;
         if (left < kBlk) {
 #pragma unroll
-          for (int e = 0; e < kBlk; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
+          for (int e = 0; e < kBlk / 2; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
         }
         float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
-        for (int e = 4; e < kBlk; e += 8) {
+        for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], sv[4 + i]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            m4[i] = e + 4 + i < kBlk ? fmaxf(fmaxf(m4[i], sv[e + i]), sv[e + 4 + i]) : fmaxf(m4[i], sv[e + i]);
+        for (int e = 8; e < kBlk / 2; e += 8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], sv[e + i], sv[e + 4 + i]);
         }
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+        tc_wait_ld_regs(x + 64);
+        tc_wait_ld_regs(x + 96);
+        if (left < kBlk) {
+#pragma unroll
+          for (int e = kBlk / 2; e < kBlk; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = kBlk / 2; e < kBlk; e += 8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m4[i] = max_nan(m4[i], sv[e + i], sv[e + 4 + i]);
+        }
+        const float mx = max_nan(max_nan(m4[0], m4[1]), m4[2], m4[3]) * p.scale_log2;
         const bool raise = mx > m_ref + kRaise;
         float alpha = 1.f;
         if (raise) {
@@ -408,6 +451,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           }
           tc_wait_st();
         }
+        // (a score that is NaN or infinite makes the row NaN, whichever pipe its exponential takes)
+        if (!(mx < INFINITY)) m_ref = NAN;
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(-ref, -ref);
         uint64_t sum2[2] = {0ull, 0ull};
@@ -418,12 +463,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           for (int e = 0; e < 32; e += 2) {
             float x0, x1;
             f2_unpack(f2_fma(f2_pack(sv[c + e], sv[c + e + 1]), sc2, nref2), x0, x1);
-            x0 = ex2_fast(x0);
-            x1 = ex2_fast(x1);
+            // part of the exponentials on the FMA pipe: the special-function unit alone would take 1024
+            // cycles for a warp's 128
+            if ((e >> 1) % kPolyOf < kPoly) {
+              exp2_poly_pair(x0, x1);
+            } else {
+              x0 = ex2_fast(x0);
+              x1 = ex2_fast(x1);
+            }
             sum2[(e >> 1) & 1] = f2_add(sum2[(e >> 1) & 1], f2_pack(x0, x1));
             pk[e >> 1] = pack_bf16x2(x0, x1);
           }
           tmem_st_32x32b_x16(s_base + (c >> 1), pk);
+          if (c == kBlk / 2 - 32) {
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t]);
+          }
         }
         float l0, l1;
         f2_unpack(f2_add(sum2[0], sum2[1]), l0, l1);
@@ -431,7 +488,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
       }
       if (!ok) break;
       // this CTA's part of the row

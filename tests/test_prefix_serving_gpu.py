@@ -184,6 +184,21 @@ def test_large_scores_and_equal_scores():
         assert torch.equal(out[:, 0], want[:, None].expand(2, 2, 64))
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("rows", [4, 80, 300])
+def test_prefix_scores_that_are_no_numbers(value, rows):
+    """A key of the prefix that is not a number spoils every row that sees it, wherever in a block it lies."""
+    for at in (0, 3, 77, 130, 255):
+        c = Case([270] * rows, 1, 1, 1, 64, 16, 264)
+        c.q = c.q.abs() + 0.1
+        c.k[c.prefix_pages.long()[at // 16], at % 16] = value
+        assert torch.isnan(c.run()).all()
+    c = Case([265] * 4, 1, 1, 1, 64, 16, 264)  # the only key of a tail
+    for b in range(4):
+        c.k[c.tables[b].long()[264 // 16], 264 % 16] = float("nan")
+    assert torch.isnan(c.run()).all()
+
+
 def test_attention_strides_streams_and_graph():
     c = Case([300, 290, 310], 2, 2, 2, 64, 16, 256, [1, 2, 2], seed=4)
     pool = c.pool()
