@@ -11,7 +11,11 @@
 //                 own copies, makes them visible to the asynchronous proxy and signals the slot full
 //   warps 8-15    two softmax warpgroups, a thread per row: read the row's 128 scores from TMEM, raise the
 //                 running maximum only when it grew by more than 2^8 (then O is rescaled in TMEM), write P
-//                 back as packed bf16 over the scores
+//                 back as packed bf16 over the scores, in two halves, so that P V of the first runs while the
+//                 second is formed. (A block costs a tile about 2000 cycles here and 1450 in the MMAs, one after
+//                 the other; the two tiles alternate. Moving 2 to 8 of 16 exponentials to the FMA pipe as
+//                 polynomials made 256 sequences behind 32768 tokens slower, 134 -> 139 to 151 us: the warps are
+//                 bound by issue and latency, not by the special-function unit.)
 // S_t at TMEM columns [128 t, +128) (P_t aliases its first half), O_t at [256 + HDP t, + HDP). MMAs of one
 // thread complete in order, so S_t of the next block may take the columns that P V_t reads, and S_t being
 // full implies that P V_t before it is in O_t.
@@ -37,27 +41,6 @@ constexpr int kBlk = 128;  // keys of a block, rows of a tile
 // warpgroups: MMA, producers, two of softmax; 512 x 128 registers at launch
 constexpr int kRegsMma = 48, kRegsLoad = 56, kRegsSoftmax = 200;
 static_assert(kRegsMma + kRegsLoad + 2 * kRegsSoftmax <= 4 * 128, "register split exceeds the launch");
-
-constexpr int kPoly = 5, kPolyOf = 16;  // pairs of exponentials on the FMA pipe
-
-// 2^x of a pair on the FMA pipe: x = n + f with n the nearest integer (added into the low mantissa bits of
-// 1.5 * 2^23) and f in [-0.5, 0.5]; 2^f by a cubic fitted to the relative error there (Remez, 7.5e-5: below
-// the bf16 rounding of P by a factor of 50); 2^n by an addition to the exponent field. x is at most
-// kRaise; below -125 the result stays at 2^-125.
-__device__ __forceinline__ void exp2_poly_pair(float& x0, float& x1) {
-  const uint64_t big = f2_pack(12582912.f, 12582912.f), nbig = f2_pack(-12582912.f, -12582912.f);
-  const uint64_t x = f2_pack(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-  const uint64_t n = f2_add(x, big);
-  const uint64_t f = f2_fma(f2_add(n, nbig), f2_pack(-1.f, -1.f), x);
-  uint64_t q = f2_fma(f2_pack(5.517166906e-02f, 5.517166906e-02f), f, f2_pack(2.426111222e-01f, 2.426111222e-01f));
-  q = f2_fma(q, f, f2_pack(6.932609855e-01f, 6.932609855e-01f));
-  q = f2_fma(q, f, f2_pack(9.999280735e-01f, 9.999280735e-01f));
-  float q0, q1, n0, n1;
-  f2_unpack(q, q0, q1);
-  f2_unpack(n, n0, n1);
-  x0 = __int_as_float(__float_as_int(q0) + (__float_as_int(n0) << 23));
-  x1 = __int_as_float(__float_as_int(q1) + (__float_as_int(n1) << 23));
-}
 
 template <int HDP>
 struct Tc {
@@ -451,7 +434,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           }
           tc_wait_st();
         }
-        // (a score that is NaN or infinite makes the row NaN, whichever pipe its exponential takes)
+        // (a score that is NaN or infinite makes the row NaN)
         if (!(mx < INFINITY)) m_ref = NAN;
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nref2 = f2_pack(-ref, -ref);
@@ -463,14 +446,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           for (int e = 0; e < 32; e += 2) {
             float x0, x1;
             f2_unpack(f2_fma(f2_pack(sv[c + e], sv[c + e + 1]), sc2, nref2), x0, x1);
-            // part of the exponentials on the FMA pipe: the special-function unit alone would take 1024
-            // cycles for a warp's 128
-            if ((e >> 1) % kPolyOf < kPoly) {
-              exp2_poly_pair(x0, x1);
-            } else {
-              x0 = ex2_fast(x0);
-              x1 = ex2_fast(x1);
-            }
+            x0 = ex2_fast(x0);
+            x1 = ex2_fast(x1);
             sum2[(e >> 1) & 1] = f2_add(sum2[(e >> 1) & 1], f2_pack(x0, x1));
             pk[e >> 1] = pack_bf16x2(x0, x1);
           }
