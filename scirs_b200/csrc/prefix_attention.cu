@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 
 }  // namespace prefix
 
-// q [B, Q, H, HD] bf16 (inner dimension contiguous) -> [B, Q, H, HD] bf16. Pools [num_pages, block_size,
+// q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape. Pools [num_pages, block_size,
 // Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
 constexpr int64_t kTcRows = 32, kTcKeys = 256;
@@ -568,7 +568,9 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   CHECK_DTYPE(q, at::kBFloat16);
   CHECK_DTYPE(k_pool, at::kBFloat16);
   CHECK_DTYPE(v_pool, at::kBFloat16);
-  TORCH_CHECK(q.dim() == 4, "q must be [B, Q, H, HD]");
+  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "q must be [B, H, HD] or [B, Q, H, HD]");
+  const auto shape = q.sizes().vec();
+  if (q.dim() == 3) q = q.unsqueeze(1);
   const int64_t B = q.size(0), Q = q.size(1), H = q.size(2), HD = q.size(3);
   TORCH_CHECK(k_pool.dim() == 4 && k_pool.sizes() == v_pool.sizes() && k_pool.is_contiguous() &&
                   v_pool.is_contiguous() && k_pool.size(3) == HD,
@@ -580,9 +582,9 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
                   reinterpret_cast<uintptr_t>(v_pool.data_ptr()) % 16 == 0,
               "pools must be 16-byte aligned");
   const bool has_ql = qlens.has_value() && qlens->defined();
-  auto ints = [&](const torch::Tensor& t, const char* what) {
-    TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == q.device(), what,
-                ": contiguous int32 on q's device");
+  auto ints = [&](torch::Tensor& t, const char* what) {
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == q.device(), what, ": int32 on q's device");
+    if (!t.is_contiguous()) t = t.contiguous();
   };
   ints(tables, "block tables");
   ints(lens, "sequence lengths");
@@ -598,7 +600,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
               " tokens is longer than its pages or than a chain");
   TORCH_CHECK(max_pages * bs < (1LL << 30) && B * Q * H < (1LL << 30), "paged attention: too large");
   c10::cuda::CUDAGuard guard(q.get_device());
-  auto out = at::empty({B, Q, H, HD}, q.options());
+  auto out = at::empty(shape, q.options());
   if (out.numel() == 0) return out;
   if (q.stride(3) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || q.stride(2) % 8 ||
       reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
@@ -656,10 +658,9 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   p.box = (HD == 64 || HD == 128) && run >= 8 ? std::min(run, prefix::kTile) : 0;
   if (tc) prefix::plan_prefix_tc(p, sms);
   const int slots = p.P + p.T;
-  auto part_o = at::empty({B * Q * H, slots, HD}, q.options().dtype(at::kFloat));
-  auto part_ml = at::empty({B * Q * H, slots, 2}, q.options().dtype(at::kFloat));
-  p.part_o = part_o.data_ptr<float>();
-  p.part_ml = part_ml.data_ptr<float>();
+  auto parts = at::empty({B * Q * H * slots * (HD + 2)}, q.options().dtype(at::kFloat));
+  p.part_o = parts.data_ptr<float>();
+  p.part_ml = p.part_o + B * Q * H * slots * HD;
   const int64_t items = Hkv * ((int64_t)p.rt_p * p.P + B * p.rt_t * p.T);
   TORCH_CHECK(items < (1LL << 31), "paged attention: too large");
   if (tc) {

@@ -144,22 +144,16 @@ def copy_pages(pools, src, dst, counts=None) -> None:
     if not pools:
         raise InferenceError("copy_pages needs at least one pool")
 
-    def host(t):
-        if isinstance(t, torch.Tensor):
-            if t.is_cuda or t.dtype != torch.int32 or t.dim() != 1:
-                raise InferenceError("page ids and counts are lists or 1-D int32 host tensors")
-            return t.contiguous()
-        return torch.tensor(list(t), dtype=torch.int32)
-
-    src, dst = host(src), host(dst)
-    counts = None if counts is None else host(counts)
-    if len(dst) != len(src) or (counts is not None and len(counts) != len(src)):
-        raise InferenceError("src, dst and counts differ in length")
+    src, dst, counts = (t if t is None or isinstance(t, torch.Tensor) else torch.tensor(list(t), dtype=torch.int32)
+                        for t in (src, dst, counts))
     bufs = [b for p in pools for b in (p.k, p.v)]
     if bufs[0].is_cuda:
         _ext.kernels().page_copy(bufs, src, dst, counts)
         K._count(1)
         return
+    for t in (src, dst, counts):
+        if t is not None and (t.is_cuda or t.dtype != torch.int32 or t.shape != (src.numel(),)):
+            raise InferenceError("page ids and counts are lists or 1-D int32 host tensors of one length")
     pages, bs = bufs[0].shape[:2]
     s, d = src.tolist(), dst.tolist()
     n = counts.tolist() if counts is not None else [bs] * len(s)

@@ -90,27 +90,26 @@ class PagedAttentionForward:
         number of query heads per cached head, any page size. bf16; the softmax and the sums are
         kept in fp32. A captured graph keeps prefix_len, and reads the tables and lengths anew.
         """
-        squeeze = q.dim() == 3
-        q4 = q.unsqueeze(1) if squeeze else q
-        c = pool.config
-        if q4.dim() != 4 or q4.shape[2:] != (self.config.num_heads, self.config.head_dim):
+        c, n = pool.config, self.config
+        if q.dim() not in (3, 4) or q.shape[-2] != n.num_heads or q.shape[-1] != n.head_dim:
             raise InferenceError("query shape does not match the configuration")
-        if self.config.num_heads % c.num_heads or self.config.head_dim != c.head_dim:
+        if n.num_heads % c.num_heads or n.head_dim != c.head_dim:
             raise InferenceError("the pool's heads do not match the configuration")
-        if not 0.0 < self._scale() < float("inf"):
+        scale = self._scale()
+        if not 0.0 < scale < float("inf"):
             raise InferenceError("scale must be positive and finite")
         if prefix_len < 0 or prefix_len > min(prefix_pages.numel(), block_tables.shape[-1]) * c.block_size:
             raise InferenceError("prefix_len is longer than the prefix's pages or a chain")
         if q.is_cuda:
-            out = _ext.kernels().paged_prefix_attention(q4.to(torch.bfloat16), pool.k, pool.v,
-                                                        block_tables.contiguous(), seq_lens.contiguous(),
-                                                        prefix_pages.contiguous(), int(prefix_len), q_lens,
-                                                        self._scale())
+            if q.dtype != torch.bfloat16:
+                q = q.to(torch.bfloat16)
+            out = _ext.kernels().paged_prefix_attention(q, pool.k, pool.v, block_tables, seq_lens, prefix_pages,
+                                                        int(prefix_len), q_lens, scale)
             K._count(2)
-        else:
-            out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens,
-                                                    self._scale())
-        return out.squeeze(1) if squeeze else out
+            return out
+        q4 = q.unsqueeze(1) if q.dim() == 3 else q
+        out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens, scale)
+        return out.reshape(q.shape)
 
     def forward_manager(self, q: torch.Tensor, manager: BlockManager, seq_ids: list[int]):
         """Decode attention for the given sequences of a BlockManager."""
