@@ -76,7 +76,8 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)((c >> 3) * Cfg<HDP>::HALF + r * 128 + ((c ^ r) & 7) * 16);
 }
 
-template <int HDP, int MT, bool TMA>
+// W: warps of an item; the CTA's four warps take one item together, or one each.
+template <int HDP, int MT, bool TMA, int W>
 __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
                                                                              const Params p) {
@@ -87,13 +88,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full_s[kWarps][C::STAGES];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part_w = warp % W;  // which of the item's warps this is
   uint64_t* full = full_s[warp];
   uint8_t* ring = smem + warp * C::WARP;
   const uint32_t ring_a = smem_u32(ring);
 
   // ---- which rows against which keys. Neighbouring items are the cached heads of the same keys, which lie
   // side by side in a page.
-  int i = blockIdx.x;
+  int i = blockIdx.x * (kWarps / W) + warp / W;
+  if (i >= p.items) {
+    wait_for_previous();
+    return;
+  }
   const int hk = i % p.Hkv;
   i /= p.Hkv;
   const bool is_prefix = i < p.P * p.rt_p;  // (rt_p = 0 when tcgen05 takes the prefix)
@@ -116,13 +122,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
   const int max_pages = is_prefix ? p.pages_max : p.max_pages;
 
   // ---- page ids: with TMA a lane holds the page and slot of one box, 32 boxes of this warp's tiles at a time
-  // (tile j of the warp begins at base + (4 j + warp) 16); with cp.async lanes 0-15 hold one tile's keys
+  // (tile j of the warp begins at base + (W j + its part) 16); with cp.async lanes 0-15 hold one tile's keys
   const int runs = TMA ? kTile / p.box : 1;  // boxes of a tile
   int base = is_prefix ? split * p.per_p : p.L & ~(kTile - 1), k1 = 0x7fffffff;
   int page = -2, at = 0, batch = 0;
   auto look_up = [&](int j) {  // TMA: the boxes of tiles j, j + 1, ..; cp.async: the keys of tile j
-    const int key = TMA ? base + (((j + lane / runs) * kWarps + warp) * kTile + lane % runs * p.box)
-                        : base + (j * kWarps + warp) * kTile + lane;
+    const int key = TMA ? base + (((j + lane / runs) * W + part_w) * kTile + lane % runs * p.box)
+                        : base + (j * W + part_w) * kTile + lane;
     const int pi = page_of(p, key);
     page = (TMA || lane < kTile) && key >= 0 && key < k1 && pi < max_pages ? pages[pi] : -2;
     at = key - pi * p.bs;
@@ -137,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     k0 = base;
     k1 = min(base + p.per_p, p.L);
   } else {
-    const Seq s = seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, threadIdx.x == 0);
+    const Seq s = seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, lane == 0 && part_w == 0);
     const int share = tail_share(p, s);
     const int first = first_key(s) + split * share;
     k0 = max(first, s.start);
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
       if (TMA) look_up(0);
     }
   }
-  const int tiles = max((k1 - base + kTile - 1) / kTile - warp + kWarps - 1, 0) / kWarps;  // of this warp
+  const int tiles = max((k1 - base + kTile - 1) / kTile - part_w + W - 1, 0) / W;  // of this warp
   if (lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
@@ -168,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
   auto copy = [&](int j, int stage) -> uint32_t {
     uint32_t valid;
     uint8_t* dst = ring + stage * 2 * C::KV;
-    const int key0 = base + (j * kWarps + warp) * kTile;
+    const int key0 = base + (j * W + part_w) * kTile;
     if (TMA) {
       if ((j - batch + 1) * runs > 32) look_up(j);
       // boxes of the whole tile, or, a lane each, of 8 keys and one half of the columns; a box that is not
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     }
     __syncwarp();
     const uint32_t vm = (uint32_t)valid_q & 0xffffu;  // the tile's keys that are used
-    const int key0 = base + (j * kWarps + warp) * kTile;
+    const int key0 = base + (j * W + part_w) * kTile;
     ++j;
     valid_q >>= 16;
     --flying;
@@ -419,10 +425,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     }
   }
 
-  // ---- join the warps (the rings are free now), write this split's part of every row
-  float* mo = reinterpret_cast<float*>(smem);  // [warp][M][HDP]
-  float* mml = mo + kWarps * M * HDP;          // [warp][M][2]
-  __syncthreads();
+  // ---- join the item's warps (their rings are free now), write this split's part of every row
+  float* mo = reinterpret_cast<float*>(W == 1 ? ring : smem);  // [part][M][HDP]
+  float* mml = mo + W * M * HDP;                               // [part][M][2]
+  const auto join = [] {
+    if (W == 1)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+  join();
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -432,23 +444,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if ((lane & 3) == 0)
-        *reinterpret_cast<float2*>(mml + (warp * M + r) * 2) = make_float2(tiles > 0 ? m_run[mt][h] : -INFINITY, l);
+        *reinterpret_cast<float2*>(mml + (part_w * M + r) * 2) = make_float2(tiles > 0 ? m_run[mt][h] : -INFINITY, l);
       if (tiles > 0 && r0 + r < r_end) {
 #pragma unroll
         for (int n = 0; n < HDP / 8; ++n)
-          *reinterpret_cast<float2*>(mo + (warp * M + r) * HDP + ((n * 8 + (lane & 3) * 2) ^ ((r & 3) * 8))) =
+          *reinterpret_cast<float2*>(mo + (part_w * M + r) * HDP + ((n * 8 + (lane & 3) * 2) ^ ((r & 3) * 8))) =
               make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
       }
     }
-  __syncthreads();
+  join();
   const int slots = p.P + p.T;
-  for (int r = warp; r < M && r0 + r < r_end; r += kWarps) {
-    float m = -INFINITY, f[kWarps], l = 0.f;
+  for (int r = part_w; r < M && r0 + r < r_end; r += W) {
+    float m = -INFINITY, f[W], l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = max_nan(m, mml[(w * M + r) * 2]);
+    for (int w = 0; w < W; ++w) m = max_nan(m, mml[(w * M + r) * 2]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       f[w] = ex2_fast(mml[(w * M + r) * 2] - ref);
       l += f[w] * mml[(w * M + r) * 2 + 1];
     }
@@ -457,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     for (int d = lane * 2; d < p.HD; d += 64) {
       float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
+      for (int w = 0; w < W; ++w)
         if (f[w] != 0.f) {  // (a warp without keys holds nothing)
           const float2 x = *reinterpret_cast<const float2*>(mo + (w * M + r) * HDP + (d ^ ((r & 3) * 8)));
           acc.x += f[w] * x.x;
@@ -479,10 +491,12 @@ CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves) {
   return make_tmap_bf16(pool, 5, ext, str, bx, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// One CTA per output row; its warps take every fourth part.
+// W warps to an output row, which take every W-th part.
+template <int W>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
-  const int row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x * (4 / W) + warp / W;
+  if (row >= p.B * p.Q * p.H) return;
   __shared__ float4 acc_s[4][32];
   __shared__ float den_s[4];
   const int bt = row / p.H, h = row - bt * p.H, b = bt / p.Q, t = bt - b * p.Q;
@@ -519,7 +533,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   float den = 0.f;
   const bool on = 4 * lane < p.HD;
 #pragma unroll 4
-  for (int j = warp; j < np + nt; j += 4) {
+  for (int j = warp % W; j < np + nt; j += W) {
     const int i = slot_of(j);
     const float2 v = *reinterpret_cast<const float2*>(ml + 2 * i);
     const float4 o = on ? *reinterpret_cast<const float4*>(po + (long)i * p.HD + 4 * lane) : acc;
@@ -532,19 +546,22 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
       acc.w += w * o.w;
     }
   }
-  acc_s[warp][lane] = acc;
-  if (lane == 0) den_s[warp] = den;
-  __syncthreads();
-  if (warp != 0 || !on) return;
+  if (W > 1) {
+    acc_s[warp][lane] = acc;
+    if (lane == 0) den_s[warp] = den;
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    const float4 o = acc_s[w][lane];
-    acc.x += o.x;
-    acc.y += o.y;
-    acc.z += o.z;
-    acc.w += o.w;
-    den += den_s[w];
+    for (int w = 1; w < W; ++w) {
+      const float4 o = acc_s[w][lane];
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+      den += den_s[w];
+    }
   }
+  if (!on) return;
   uint2 out = make_uint2(0u, 0u);
   if (den != 0.f) {
     const float inv = 1.f / den;
@@ -560,6 +577,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
 constexpr int64_t kTcRows = 32, kTcKeys = 256;
 constexpr int64_t kMinKeys = 128;
+constexpr int kFewParts = 8;
 
 torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
                                      torch::Tensor lens, torch::Tensor pages, int64_t L,
@@ -662,7 +680,10 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   p.part_o = parts.data_ptr<float>();
   p.part_ml = p.part_o + B * Q * H * slots * HD;
   const int64_t items = Hkv * ((int64_t)p.rt_p * p.P + B * p.rt_t * p.T);
-  TORCH_CHECK(items < (1LL << 31), "paged attention: too large");
+  TORCH_CHECK(items < (1LL << 30), "paged attention: too large");
+  p.items = (int)items;
+  // many short tails (no longer than an item's smallest share, more than two rounds of CTAs): a warp each
+  const bool solo = mt == 1 && p.rt_p == 0 && span <= kMinKeys && items > ctas;
   if (tc) {
     prefix::launch_prefix_tc(p, cur_stream());
   }
@@ -672,23 +693,38 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
     map_k = prefix::pool_map(p, p.k, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
     map_v = prefix::pool_map(p, p.v, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
   }
-#define SCIRS_ITEMS(HDP_, MT_, TMA_)                                                                                \
-  {                                                                                                                 \
-    auto kern = prefix::item_kernel<HDP_, MT_, TMA_>;                                                               \
-    constexpr int smem = prefix::Cfg<HDP_>::smem(MT_);                                                              \
-    set_max_smem((const void*)kern, smem);                                                                          \
-    prefix::launch(kern, (unsigned)items, prefix::kThreads, smem, st, tc, map_k, map_v, p);                         \
+#define SCIRS_ITEMS(HDP_, MT_, TMA_, W_)                                                                             \
+  {                                                                                                                  \
+    auto kern = prefix::item_kernel<HDP_, MT_, TMA_, W_>;                                                            \
+    constexpr int smem = prefix::Cfg<HDP_>::smem(MT_), each = prefix::kWarps / W_;                                   \
+    set_max_smem((const void*)kern, smem);                                                                           \
+    prefix::launch(kern, (unsigned)((items + each - 1) / each), prefix::kThreads, smem, st, tc, map_k, map_v, p);    \
   }
-#define SCIRS_ITEMS_MT(HDP_, TMA_) \
-  if (mt == 1) SCIRS_ITEMS(HDP_, 1, TMA_) else SCIRS_ITEMS(HDP_, 2, TMA_)
+#define SCIRS_ITEMS_MT(HDP_, TMA_)                  \
+  if (solo)                                         \
+    SCIRS_ITEMS(HDP_, 1, TMA_, 1)                   \
+  else if (mt == 1)                                 \
+    SCIRS_ITEMS(HDP_, 1, TMA_, 4)                   \
+  else                                              \
+    SCIRS_ITEMS(HDP_, 2, TMA_, 4)
   if (p.box > 0) {
-    if (HD == 64) SCIRS_ITEMS_MT(64, true) else SCIRS_ITEMS_MT(128, true)
+    if (HD == 64) {
+      SCIRS_ITEMS_MT(64, true)
+    } else {
+      SCIRS_ITEMS_MT(128, true)
+    }
+  } else if (HD <= 64) {
+    SCIRS_ITEMS_MT(64, false)
   } else {
-    if (HD <= 64) SCIRS_ITEMS_MT(64, false) else SCIRS_ITEMS_MT(128, false)
+    SCIRS_ITEMS_MT(128, false)
   }
 #undef SCIRS_ITEMS_MT
 #undef SCIRS_ITEMS
-  prefix::launch(prefix::combine_kernel, (unsigned)(B * Q * H), 128, 0, st, true, p);
+  // four warps to a row where its parts are many, one where they are few
+  if (slots > kFewParts)
+    prefix::launch(prefix::combine_kernel<4>, (unsigned)(B * Q * H), 128, 0, st, true, p);
+  else
+    prefix::launch(prefix::combine_kernel<1>, (unsigned)((B * Q * H + 3) / 4), 128, 0, st, true, p);
   return out;
 }
 

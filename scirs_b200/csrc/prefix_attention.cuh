@@ -24,6 +24,7 @@ struct Params {
   int P, T;             // splits of the prefix and of a tail, and their slots: 0 .. P - 1, P .. P + T - 1
   int per_p, rt_p, rt_t;  // item_kernel: keys of a prefix split; row tiles of the prefix (0: tcgen05 takes it), of a tail
   int pages_max;        // pages of the prefix
+  int items;            // of item_kernel
   int box;              // keys of a TMA box (0: cp.async)
   uint32_t bs_mul;      // division by bs (see page_of)
   int bs_shift;

@@ -123,6 +123,10 @@ CASES = [
     pytest.param([520 + i for i in range(129)], 1, 1, 1, 64, 16, 512, None, id="129_rows"),
     pytest.param([4000 + i for i in range(6)], 1, 16, 7, 64, 128, 3999, None, id="sixteen_heads"),
     pytest.param([5000 + 3 * i for i in range(40)], 1, 1, 16, 128, 16, 4990, None, id="640_rows_long"),
+    # more short tails than two rounds of CTAs
+    pytest.param([291 + i % 20 for i in range(130)], 1, 8, 1, 64, 16, 290, None, id="1040_short_tails"),
+    pytest.param([1 + i % 30 for i in range(100)], 3, 8, 2, 128, 5, 0, [1 + i % 3 for i in range(100)], id="800_tails_no_prefix"),
+    pytest.param([0 if i % 7 == 0 else 20 + i % 90 for i in range(130)], 2, 8, 1, 128, 8, 17, [i % 3 for i in range(130)], id="short_tails_shorter_than_prefix"),
 ]
 
 
