@@ -575,8 +575,15 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 // q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape. Pools [num_pages, block_size,
 // Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
-constexpr int64_t kTcRows = 32, kTcKeys = 256;
-constexpr int64_t kMinKeys = 128;
+// tcgen05 takes the prefix from kTcKeys keys on if more than kTcRows rows share a cached head, and from kTcLong
+// keys on always (8 cached heads of 128, tails of 128, mma.sync -> tcgen05: 24 rows, 1024 keys 15.8 -> 14.8 us,
+// 8192 keys 37 -> 25 us; 16 rows, 8192 keys 21 -> 23 us, 65536 keys 66 -> 60 us; 16 rows of heads of 64, 1024 keys
+// 10.8 -> 13.0 us).
+constexpr int64_t kTcRows = 16, kTcKeys = 512, kTcLong = 32768;
+// Keys of an item, at least (16 rows, 1024 keys of the prefix: 256 instead of 128 takes 12.8 us, not 10.8), and
+// parts of a row's prefix, at most, where they fill the device (8192 keys in 32 parts instead of 64: 22 -> 15 us).
+constexpr int64_t kMinKeys = 128, kParts = 32;
+// Up to here a warp joins a row's parts, above four do (2048 rows of 20 parts: 9 us with four).
 constexpr int kFewParts = 8;
 
 torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
@@ -650,7 +657,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
 
   const int64_t seq_rows = Q * p.G, rows = B * seq_rows;
   const int sms = num_sms(q.get_device());
-  const bool tc = L >= kTcKeys && rows > kTcRows;
+  const bool tc = (L >= kTcKeys && rows > kTcRows) || L >= kTcLong;
   const int mt = std::max(L > 0 && !tc ? rows : 0, seq_rows) > 16 ? 2 : 1;
   p.rt_p = L > 0 && !tc ? (int)((rows + 16 * mt - 1) / (16 * mt)) : 0;
   p.rt_t = (int)((seq_rows + 16 * mt - 1) / (16 * mt));
@@ -658,19 +665,16 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   p.bs_shift = 31;
   while ((1LL << (p.bs_shift - 31)) < bs) ++p.bs_shift;
   p.bs_mul = (uint32_t)(((1ULL << p.bs_shift) + bs - 1) / bs);
-  // two rounds of CTAs, of at least kMinKeys keys each
+  // tails: two rounds of CTAs, of at least kMinKeys keys each
   const int64_t ctas = 2LL * sms * (HD <= 64 ? prefix::Cfg<64>::ctas(mt) : prefix::Cfg<128>::ctas(mt));
   const int64_t span = max_pages * bs - L;
-  const auto splits = [&](int64_t tiles, int64_t keys) {
-    return std::max<int64_t>(1, std::min(ctas / std::max<int64_t>(1, Hkv * tiles), (keys + kMinKeys - 1) / kMinKeys));
-  };
   p.P = 0;
   if (p.rt_p > 0) {
-    const int64_t n = splits(p.rt_p, L);
+    const int64_t n = std::min((L + kMinKeys - 1) / kMinKeys, std::max<int64_t>(kParts, 2 * sms / (Hkv * p.rt_p)));
     p.per_p = (int)(((L + n - 1) / n + prefix::kTile - 1) / prefix::kTile * prefix::kTile);
     p.P = (int)((L + p.per_p - 1) / p.per_p);
   }
-  p.T = (int)splits(B * p.rt_t, span);
+  p.T = (int)std::max<int64_t>(1, std::min(ctas / (Hkv * B * p.rt_t), (span + kMinKeys - 1) / kMinKeys));
   // boxes of a power of two that divides the page size, at least the 8 rows of the swizzle
   const int run = p.bs & -p.bs;
   p.box = (HD == 64 || HD == 128) && run >= 8 ? std::min(run, prefix::kTile) : 0;
