@@ -6,7 +6,9 @@
 // memory copy of many runs: 2 x bytes of traffic and nothing to compute. The page ids and the pools'
 // addresses travel as kernel parameters (no table in device memory has to be written first, and a
 // captured graph keeps them); a CTA takes a chunk of 256 x U 16-byte vectors of one run at a time, U of
-// them in flight per thread.
+// them in flight per thread. Measured: 680 pages of 32 KB in 32 pools (1.43 GB read and written) 249 us,
+// 5.7 TB/s, 0.87 of a plain device copy's rate; 64 partly filled pages in 48 pools (107 MB) 21 us; 8 in 24
+// pools 2.7 us on the device, 8 us a call, bound by the call on the host.
 //
 // Reference parity: scirs2-neural/src/inference/block_manager.rs:196-280 (page chains and the shared
 // prefix cache; pages are never copied there).

@@ -26,6 +26,11 @@
 //   2: a row tile is 128 rows; tile t takes every other key block of the same rows (few rows: two
 //      independent chains keep the loads and the tensor core busy), and writes a part of its own
 //
+// Measured: 1024 rows of each of 8 cached heads of 128 against 32768 keys (137 GFLOP) 134 us, 1.0 PFLOP/s, 0.62
+// of the measured bf16 rate, the tensor pipe active 49 % of the time; 80 rows against 100003 keys (410 MB) 78 us,
+// 5.2 TB/s; 256 rows against 8192 keys 22 us, of which about 10 are the start (lengths, queries, first block, code
+// fetched for the first time) and the end of the four blocks that a CTA gets.
+//
 // Work is laid out evenly: the blocks of all row tiles end to end are cut into equal shares, one per CTA,
 // so a CTA may finish one row tile and begin the next; its part of a row tile goes to the slot given by how
 // many CTAs before it met that tile. Every wait is bounded (common.cuh).
