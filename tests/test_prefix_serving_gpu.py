@@ -123,6 +123,10 @@ CASES = [
     pytest.param([520 + i for i in range(129)], 1, 1, 1, 64, 16, 512, None, id="129_rows"),
     pytest.param([4000 + i for i in range(6)], 1, 16, 7, 64, 128, 3999, None, id="sixteen_heads"),
     pytest.param([5000 + 3 * i for i in range(40)], 1, 1, 16, 128, 16, 4990, None, id="640_rows_long"),
+    pytest.param([600, 520, 0, 513, 700, 640], 1, 2, 8, 128, 16, 513, None, id="48_rows_prefix_inside_page"),
+    pytest.param([33000], 1, 1, 1, 64, 128, 32990, None, id="one_row_long"),
+    pytest.param([33000, 40, 32800], 2, 1, 2, 128, 8, 32780, [2, 1, 1], id="twelve_rows_long"),
+    pytest.param([600 + i for i in range(9)], 1, 1, 2, 72, 16, 597, None, id="tc_head_dim_72"),
     # more short tails than two rounds of CTAs
     pytest.param([291 + i % 20 for i in range(130)], 1, 8, 1, 64, 16, 290, None, id="1040_short_tails"),
     pytest.param([1 + i % 30 for i in range(100)], 3, 8, 2, 128, 5, 0, [1 + i % 3 for i in range(100)], id="800_tails_no_prefix"),
@@ -154,16 +158,17 @@ def test_attention_agrees_with_the_decode_kernel():
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf"), -3.3895e38])
-@pytest.mark.parametrize("L", [0, 90])
+@pytest.mark.parametrize("L", [0, 90, 600])
 def test_masked_drafts_do_not_reach_earlier_queries(value, L):
     """The last drafted token's keys and values are not numbers: the queries before it do not see them."""
-    c = Case([100, 97], 4, 1, 2, 64, 16, L, seed=3)
-    page = c.tables[0].long()[99 // 16]
-    c.k[page, 99 % 16], c.v[page, 99 % 16] = value, value
+    n = max(100, L + 10)
+    c = Case([n, n - 3] + [n - 2] * 3, 4, 1, 2, 64, 16, L, seed=3)
+    page = c.tables[0].long()[(n - 1) // 16]
+    c.k[page, (n - 1) % 16], c.v[page, (n - 1) % 16] = value, value
     out = c.run()
     seen = torch.isfinite(out).all(-1).cpu()
-    assert seen[0, :3].all() and seen[1].all()
-    c.k[page, 99 % 16], c.v[page, 99 % 16] = 0.0, 0.0
+    assert seen[0, :3].all() and seen[1:].all()
+    c.k[page, (n - 1) % 16], c.v[page, (n - 1) % 16] = 0.0, 0.0
     o, a = c.exact()
     err = (out.cpu().double() - o).abs()[:, :3]
     assert (err <= (2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * a)[:, :3]).all()
@@ -192,8 +197,8 @@ def test_large_scores_and_equal_scores():
 @pytest.mark.parametrize("rows", [4, 80, 300])
 def test_prefix_scores_that_are_no_numbers(value, rows):
     """A key of the prefix that is not a number spoils every row that sees it, wherever in a block it lies."""
-    for at in (0, 3, 77, 130, 255):
-        c = Case([270] * rows, 1, 1, 1, 64, 16, 264)
+    for L, at in [(264, 0), (264, 130), (264, 263), (700, 0), (700, 3), (700, 77), (700, 130), (700, 500), (700, 699)]:
+        c = Case([L + 6] * rows, 1, 1, 1, 64, 16, L)
         c.q = c.q.abs() + 0.1
         c.k[c.prefix_pages.long()[at // 16], at % 16] = value
         assert torch.isnan(c.run()).all()
@@ -203,20 +208,22 @@ def test_prefix_scores_that_are_no_numbers(value, rows):
     assert torch.isnan(c.run()).all()
 
 
-def test_attention_strides_streams_and_graph():
-    c = Case([300, 290, 310], 2, 2, 2, 64, 16, 256, [1, 2, 2], seed=4)
+@pytest.mark.parametrize("L,copies", [(256, 1), (640, 3)])
+def test_attention_strides_streams_and_graph(L, copies):
+    c = Case([L + 44, L + 34, L + 54] * copies, 2, 2, 2, 64, 16, L, [1, 2, 2] * copies, seed=4)
+    B = 3 * copies
     pool = c.pool()
     want = c.run(pool=pool)
     c.check(want)
     # q as a slice of a fused projection's output; an odd offset; tables of a wider matrix
     H = c.Hkv * c.G
-    fused = torch.randn(3, 2, 3, H, 64, device=DEV).to(torch.bfloat16)
+    fused = torch.randn(B, 2, 3, H, 64, device=DEV).to(torch.bfloat16)
     fused[:, :, 1] = c.q.to(DEV)
     assert torch.equal(c.run(fused[:, :, 1], pool), want)
     odd = torch.empty(c.q.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view_as(c.q)
     odd.copy_(c.q)
     assert torch.equal(c.run(odd, pool), want)
-    wide = torch.full((3, c.tables.shape[1] + 9), 12345, dtype=torch.int32, device=DEV)
+    wide = torch.full((B, c.tables.shape[1] + 9), 12345, dtype=torch.int32, device=DEV)
     wide[:, : c.tables.shape[1]] = c.tables.to(DEV)
     assert torch.equal(c.run(pool=pool, tables=wide[:, : c.tables.shape[1]]), want)
     s = torch.cuda.Stream()
@@ -225,7 +232,7 @@ def test_attention_strides_streams_and_graph():
         assert torch.equal(c.run(pool=pool), want)
     # captured twice, replayed on two streams at once with other lengths than at the capture
     args = [t.to(DEV) for t in (c.q, c.tables, c.lens, c.prefix_pages, c.qlens)]
-    args[2].fill_(260)
+    args[2].fill_(L + 4)
     graphs, outs = [], []
     for _ in range(2):
         gr = torch.cuda.CUDAGraph()
@@ -282,7 +289,25 @@ def test_attention_bad_pages_and_lengths_are_reported():
     c.check(out)
 
 
+@pytest.mark.parametrize("bs", [5, 16])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+def test_bad_prefix_pages_are_reported_by_the_long_prefix_path(bs, bad):
+    c = Case([650 + i for i in range(20)], 1, 2, 2, 64, bs, 640)
+    c.k, c.v = torch.nan_to_num(c.k), torch.nan_to_num(c.v)
+    c.check(c.run())
+    c.prefix_pages[7] = bad
+    out = c.run()
+    with pytest.raises(RuntimeError, match="bounds"):
+        _ext.check_status(0)
+    assert torch.isfinite(out).all()
+
+
 def test_attention_refuses():
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        c = Case([40, 33], 1, 2, 2, 64, 16, 32)
+        c.att.config.scale = scale
+        with pytest.raises(RuntimeError, match="scale"):
+            c.run()
     c = Case([40, 33], 1, 2, 2, 64, 16, 32)
     pool = c.pool()
     q, t, n, p = c.q.to(DEV), c.tables.to(DEV), c.lens.to(DEV), c.prefix_pages.to(DEV)
