@@ -10,7 +10,7 @@
 //
 // What it costs: 2 n gathered values, then ONE row of p and one of q a sequence, read once: bound by
 // memory for a batch, by the chain of dependent loads for one sequence. A cluster of 8 CTAs takes a
-// sequence; each of its 64 warps sums a contiguous segment of the row, the 64 sums are exchanged
+// sequence (one CTA, where a batch is large and its rows are short); each of its 64 warps sums a contiguous segment of the row, the 64 sums are exchanged
 // through distributed shared memory, and the CTA that owns the segment with the answer reads that
 // segment again (from L2) to find it. The answer is a whole number that must not depend on rounding
 // next to a border, so products, differences and sums are formed in 64 bits (u q and p - q of 32-bit
@@ -34,7 +34,7 @@ namespace verify {
 namespace cg = cooperative_groups;
 
 constexpr int kCluster = 8, kThreads = 256, kWarps = kThreads / 32;
-constexpr int kSegs = kCluster * kWarps;
+constexpr int kMaxSegs = kCluster * kWarps;  // two to a lane
 
 struct Params {
   const void *target, *draft;  // draft may be null: it is certain of its tokens
@@ -84,14 +84,16 @@ struct Row {
 };
 
 // VEC: the rows begin at multiples of 16 bytes, so that a lane reads 16 of them at a time.
-template <typename T, bool VEC>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 5) verify_kernel(const Params a) {
+// CL: CTAs of a sequence.
+template <typename T, bool VEC, int CL>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kThreads, 5) verify_kernel(const Params a) {
+  constexpr int kSegs = CL * kWarps;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int kept_s, hit_s, last_s;
   __shared__ double seg_sum[kWarps];  // read by the whole cluster
-  __shared__ double all_sum[kSegs], scan_s[kThreads], wsum[kWarps];
+  __shared__ double all_sum[kMaxSegs], scan_s[kThreads], wsum[kWarps];
 
   const T* tb = reinterpret_cast<const T*>(a.target) + b * a.ts_b;
   const T* db = a.draft != nullptr ? reinterpret_cast<const T*>(a.draft) + b * a.ds_b : nullptr;
@@ -163,10 +165,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 5) 
       if (lane == 0) seg_sum[warp] = s;
     }
     cluster.sync();
-    if (tid < kSegs) all_sum[tid] = cluster.map_shared_rank(seg_sum, tid / kWarps)[tid % kWarps];
+    if (tid < kMaxSegs) all_sum[tid] = tid < kSegs ? cluster.map_shared_rank(seg_sum, tid / kWarps)[tid % kWarps] : 0.0;
     __syncthreads();
     cluster.barrier_arrive();  // (waited for before seg_sum is written again, and before this CTA leaves)
-    // prefix sums of the 64 segments, two to a lane; every warp computes the same
+    // prefix sums of the segments, two to a lane; every warp computes the same
     const double s0 = all_sum[2 * lane], s1 = all_sum[2 * lane + 1];
     const double inc = warp_scan_d(s0 + s1, lane);
     double exc = __shfl_up_sync(0xffffffffu, inc, 1);
@@ -282,20 +284,27 @@ std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10:
   a.n = (int)n;
   a.V = (int)V;
   a.threshold = threshold;
-  const dim3 grid(verify::kCluster, (unsigned)B);
   const auto aligned = [](const torch::Tensor& t) {
     const int64_t v = 16 / t.element_size();
     return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % v == 0 && t.stride(1) % v == 0;
   };
   // 16 bytes a lane where a warp's segment gives every lane four of them: 256 rows of 131072 fp32 82 -> 66 us
   // against single values, but 64 rows of 50257 bf16 12.5 -> 17.4 us (99 vectors for the 32 lanes of a warp)
-  const bool vec = V >= (int64_t)verify::kSegs * 32 * 4 * (16 / target.element_size()) && aligned(target) &&
+  const bool vec = V >= (int64_t)verify::kMaxSegs * 32 * 4 * (16 / target.element_size()) && aligned(target) &&
                    (!has_draft || aligned(*draft));
-#define SCIRS_VERIFY(T_)                                                                                      \
-  if (vec)                                                                                                    \
-    verify::verify_kernel<T_, true><<<grid, verify::kThreads, 0, cur_stream()>>>(a);                          \
-  else                                                                                                        \
-    verify::verify_kernel<T_, false><<<grid, verify::kThreads, 0, cur_stream()>>>(a);                         \
+  // one CTA a sequence where a cluster's eight would queue up for longer than it reads the row: that grows with B
+  // in rounds of CTAs, the row with V. Eight -> one: 256 rows of 2505 16.0 -> 7.4 us, of 32769 32 -> 29, 128 of 8191
+  // 11.0 -> 11.1, 64 of 256 5.7 -> 4.8, but 64 of 8191 7.0 -> 10.8 and 32 of 2505 5.2 -> 6.8.
+  const bool solo = !vec && 2 * V <= B * B;
+#define SCIRS_VERIFY_CL(T_, V_, CL_) \
+  verify::verify_kernel<T_, V_, CL_><<<dim3(CL_, (unsigned)B), verify::kThreads, 0, cur_stream()>>>(a)
+#define SCIRS_VERIFY(T_)                              \
+  if (vec)                                            \
+    SCIRS_VERIFY_CL(T_, true, verify::kCluster);      \
+  else if (solo)                                      \
+    SCIRS_VERIFY_CL(T_, false, 1);                    \
+  else                                                \
+    SCIRS_VERIFY_CL(T_, false, verify::kCluster);     \
   break;
   switch (target.scalar_type()) {
     case at::kFloat:
@@ -308,6 +317,7 @@ std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10:
       TORCH_CHECK(false, "probabilities must be fp32, bf16 or fp16, got ", target.scalar_type());
   }
 #undef SCIRS_VERIFY
+#undef SCIRS_VERIFY_CL
   SCIRS_CHECK_LAUNCH();
   return {accepted, out};
 }

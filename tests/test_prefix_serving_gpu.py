@@ -418,7 +418,8 @@ def _verify_exact(p, q, x, u, lens, threshold):
     (1, 4, 50257, torch.float32, False, True, 0, 0.0), (7, 1, 1, torch.float32, False, True, 0, 0.0),
     (33, 5, 50257, torch.bfloat16, True, True, 47, 0.0), (16, 3, 1000, torch.float16, True, False, 3, 0.1),
     (64, 40, 63, torch.float32, True, True, 1, 0.0), (5, 0, 777, torch.float32, False, False, 0, 0.0),
-    (9, 8, 131072, torch.float32, False, True, 0, 0.3), (300, 2, 65, torch.bfloat16, False, True, 0, 0.0)])
+    (9, 8, 131072, torch.float32, False, True, 0, 0.3), (300, 2, 65, torch.bfloat16, False, True, 0, 0.0),
+    (256, 3, 32768, torch.float32, True, True, 0, 0.0), (200, 4, 9001, torch.float16, True, False, 2, 0.2)])
 def test_verify_matches_the_definition(B, n, V, dtype, ragged, with_draft, pad, threshold):
     g = torch.Generator().manual_seed(V + n)
     lp = torch.randn(B, n + 1, V, generator=g) * 2
