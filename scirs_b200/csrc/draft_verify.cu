@@ -10,11 +10,11 @@
 //
 // What it costs: 2 n gathered values, then ONE row of p and one of q a sequence, read once: bound by
 // memory for a batch, by the chain of dependent loads for one sequence. A cluster of 8 CTAs takes a
-// sequence (one CTA, where a batch is large and its rows are short); each of its 64 warps sums a contiguous segment of the row, the 64 sums are exchanged
-// through distributed shared memory, and the CTA that owns the segment with the answer reads that
-// segment again (from L2) to find it. The answer is a whole number that must not depend on rounding
-// next to a border, so products, differences and sums are formed in 64 bits (u q and p - q of 32-bit
-// values are exact there) in a fixed order.
+// sequence (one CTA, where a batch is large and its rows are short); each of its 64 warps sums a
+// contiguous segment of the row, the 64 sums are exchanged through distributed shared memory, and the CTA
+// that owns the segment with the answer reads that segment again (from L2) to find it. The answer is a
+// whole number that must not depend on rounding next to a border, so products, differences and sums are
+// formed in 64 bits (u q and p - q of 32-bit values are exact there) in a fixed order.
 //
 // Measured: 256 sequences of 8 drafts over 131072 tokens (246 MB of rows) 61 us, 4.0 TB/s, 0.61 of the device's
 // copy rate: a CTA reads its 131 KB only after the accepted drafts are known and is idle in the two exchanges
@@ -253,7 +253,7 @@ std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10:
   auto rows = [&](const torch::Tensor& t, const char* what, int64_t count) {
     TORCH_CHECK(t.device() == target.device() && t.scalar_type() == target.scalar_type() && t.dim() == 3 &&
                     t.size(0) == B && t.size(1) == count && t.size(2) == V && (V == 1 || t.stride(2) == 1),
-                what, " must be [", num(B), ", ", num(count), ", ", num(V), "] with contiguous rows, typed as the target's");
+                what, " must be [", num(B), ", ", num(count), ", ", num(V), "] with contiguous rows of the target's type");
   };
   rows(target, "target probabilities", n + 1);
   const bool has_draft = draft.has_value() && draft->defined(), has_lens = lens.has_value() && lens->defined();

@@ -22,7 +22,8 @@ struct Params {
   int B, Q, H, Hkv, G, HD, bs;
   int L;                // tokens of the prefix
   int P, T;             // splits of the prefix and of a tail, and their slots: 0 .. P - 1, P .. P + T - 1
-  int per_p, rt_p, rt_t;  // item_kernel: keys of a prefix split; row tiles of the prefix (0: tcgen05 takes it), of a tail
+  int per_p;            // item_kernel: keys of a prefix split
+  int rt_p, rt_t;       // item_kernel: row tiles of the prefix (0: tcgen05 takes it), of a tail
   int pages_max;        // pages of the prefix
   int items;            // of item_kernel
   int box;              // keys of a TMA box (0: cp.async)
@@ -109,11 +110,11 @@ __device__ __forceinline__ const bf16* prefix_query(const Params& p, int r, int 
   return p.q + b * p.q_sb + t * p.q_st + (long)(hk * p.G + r % p.G) * p.q_sh;
 }
 
-__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3, int c4) {
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3, int c4) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
-      "[%2];" ::"r"(smem_u32(smem_dst)),
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(smem_dst)),
       "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
@@ -122,8 +123,8 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
 CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves);
 
 // The kernels of one call overlap at their ends: each may start when the one before it has started all its
-// CTAs, and waits for its completion where it needs it. Every kernel waits before it ends, so that a kernel
-// behind it finds all of them done.
+// CTAs, and waits for its completion where it needs it, at the latest before it ends itself, so that what comes
+// behind the last one finds all of them done. The first one waits for everything in front of the call.
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
           int page = 0;
           if (lane * box < kBlk) {
             page = p.pages[page_of(p, key)];
-            if (!input_in_range(page, p.num_pages, p.st, 96)) page = 0;  // (reported: what is read in its place is void)
+            if (!input_in_range(page, p.num_pages, p.st, 96)) page = 0;  // (reported)
           }
           if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
             ok = false;

@@ -108,7 +108,8 @@ class PagedAttentionForward:
             K._count(2)
             return out
         q4 = q.unsqueeze(1) if q.dim() == 3 else q
-        out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens, scale)
+        out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens,
+                                                scale)
         return out.reshape(q.shape)
 
     def forward_manager(self, q: torch.Tensor, manager: BlockManager, seq_ids: list[int]):

@@ -425,7 +425,9 @@ def test_verify_matches_the_definition(B, n, V, dtype, ragged, with_draft, pad, 
     lp = torch.randn(B, n + 1, V, generator=g) * 2
     lq = lp[:, :n] + torch.randn(B, n, V, generator=g) * 0.5
     p, q = torch.softmax(lp, -1).to(dtype), torch.softmax(lq, -1).to(dtype)
-    x = torch.multinomial(q.float().view(B * n, V), 1, generator=g).view(B, n) if n else torch.zeros(B, 0, dtype=torch.int64)
+    x = torch.zeros(B, 0, dtype=torch.int64)
+    if n:
+        x = torch.multinomial(q.float().view(B * n, V), 1, generator=g).view(B, n)
     u = torch.rand(B, n + 1, generator=g)
     lens = torch.randint(0, n + 1, (B,), generator=g).to(torch.int32) if ragged else None
     pd = torch.full((B, n + 1, V + pad), float("nan"), dtype=dtype, device=DEV)[..., :V]
@@ -556,7 +558,8 @@ def test_forked_sequences_over_shared_pages():
     write([3, 0], [3, 20])
     check([0, 1, 2, 3])
     assert bm.compact()
-    assert max(p for s in range(4) for p in bm.sequence_page_chain(s)) < sum(1 for p in range(64) if pools[0].ref_count(p))
+    in_use = sum(1 for p in range(64) if pools[0].ref_count(p))
+    assert max(p for s in range(4) for p in bm.sequence_page_chain(s)) < in_use
     check([0, 1, 2, 3])
     write([1, 2], [9, 1])
     check([2, 1])
