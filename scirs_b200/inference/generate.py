@@ -17,6 +17,8 @@ page management follows scirs2-neural/src/inference/block_manager.rs.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import torch
 
 from .. import _ext
@@ -59,6 +61,16 @@ class GPTGenerator:
                 pid = int(mgr._bt_host[row, ps // bs])
                 self.pools[l].k[pid, ps % bs] = k[i]
                 self.pools[l].v[pid, ps % bs] = v[i]
+
+    @contextmanager
+    def _undone(self, seq_ids: list[int], lens: list[int]):
+        """Sequences that have grown go back to their lengths `lens` if the block does not end well."""
+        try:
+            yield
+        except BaseException:
+            for s, n in zip(seq_ids, lens):
+                self.manager.truncate_sequence(s, n)
+            raise
 
     # ----------------------------------------------------------- API
     @torch.no_grad()
@@ -143,20 +155,21 @@ class GPTGenerator:
         lens = [self.manager.seq_len(s) for s in seq_ids]
         posn = torch.tensor(lens, dtype=torch.long, device=dev)
         rows, pos = self.manager.reserve(seq_ids, [1] * n)
-        self.manager.sync()
-        bt, sl, pages, shared = self._cache_of(seq_ids)
+        with self._undone(seq_ids, lens):
+            self.manager.sync()
+            bt, sl, pages, shared = self._cache_of(seq_ids)
 
-        def attend(q, pool):
-            if shared:  # forked sequences: the pages they all begin with are read once
-                return self.attn.forward_shared_prefix(q, pool, bt, sl, pages, shared)
-            return self.attn.forward_batch(q.contiguous(), pool, bt, sl)
+            def attend(q, pool):
+                if shared:  # forked sequences: the pages they all begin with are read once
+                    return self.attn.forward_shared_prefix(q, pool, bt, sl, pages, shared)
+                return self.attn.forward_batch(q.contiguous(), pool, bt, sl)
 
-        lg = self._decode(toks, posn, rows, pos, attend)
-        if temperature > 0:
-            nxt = torch.multinomial(torch.softmax(lg / temperature, -1), 1, generator=generator).view(-1)
-        else:
-            nxt = torch.argmax(lg, dim=-1)
-        out = [int(t) for t in nxt.tolist()]
+            lg = self._decode(toks, posn, rows, pos, attend)
+            if temperature > 0:
+                nxt = torch.multinomial(torch.softmax(lg / temperature, -1), 1, generator=generator).view(-1)
+            else:
+                nxt = torch.argmax(lg, dim=-1)
+            out = [int(t) for t in nxt.tolist()]
         for s, t in zip(seq_ids, out):
             self.last_token[s] = t
         return out
@@ -168,10 +181,11 @@ class GPTGenerator:
         (drafts[i], any number of them), keep the drafts that the model confirms, and return per
         sequence those and the token that follows, which becomes its pending one.
 
-        draft_probs fp32 [B, n, vocab], n the largest number of drafts, holds the distributions that
-        the drafts were drawn from (None: the draft is certain of them); uniforms fp32 [B, n + 1] the
-        random numbers (default: drawn here). Temperature 0 keeps the drafts that equal the model's
-        own choice. The cache of rejected drafts is given back (speculative.verify_drafts)."""
+        draft_probs [B, n, vocab] (fp32, bf16 or fp16), n the largest number of drafts, holds the
+        distributions that the drafts were drawn from (None: the draft is certain of them); uniforms
+        fp32 [B, n + 1] the random numbers (default: drawn here); both on the model's device.
+        Temperature 0 keeps the drafts that equal the model's own choice. The cache of rejected drafts
+        is given back (speculative.verify_drafts). A call that raises leaves every sequence as it was."""
         B, dev, mgr = len(seq_ids), self.m.device, self.manager
         if len(drafts) != B:
             raise InferenceError("one list of drafts per sequence")
@@ -185,44 +199,52 @@ class GPTGenerator:
         fed = [t for s, d in zip(seq_ids, drafts) for t in (self.last_token[s], *d)]
         if any(not 0 <= t < self.cfg.vocab_size for t in fed):
             raise InferenceError("drafted token outside the vocabulary")
-        if draft_probs is not None and draft_probs.shape != (B, Q - 1, self.cfg.vocab_size):
-            raise InferenceError(f"draft_probs must be [{B}, {Q - 1}, {self.cfg.vocab_size}]")
-        if uniforms is not None and uniforms.shape != (B, Q):
-            raise InferenceError(f"uniforms must be [{B}, {Q}]")
+        place = self.pools[0].k.device
+        if draft_probs is not None:
+            if draft_probs.shape != (B, Q - 1, self.cfg.vocab_size):
+                raise InferenceError(f"draft_probs must be [{B}, {Q - 1}, {self.cfg.vocab_size}]")
+            if draft_probs.dtype not in (torch.float32, torch.bfloat16, torch.float16) or draft_probs.device != place:
+                raise InferenceError(f"draft_probs must be fp32, bf16 or fp16 on {place}")
+        if uniforms is not None:
+            if uniforms.shape != (B, Q):
+                raise InferenceError(f"uniforms must be [{B}, {Q}]")
+            if uniforms.dtype != torch.float32 or uniforms.device != place:
+                raise InferenceError(f"uniforms must be fp32 on {place}")
         toks = torch.tensor(fed, dtype=torch.long, device=dev)
         posn = torch.tensor([a + i for a, c in zip(lens, counts) for i in range(c)], dtype=torch.long, device=dev)
         at = torch.tensor([b * Q + i for b, c in enumerate(counts) for i in range(c)], dtype=torch.long, device=dev)
         rows, pos = mgr.reserve(seq_ids, counts)
-        mgr.sync()
-        bt, sl, pages, shared = self._cache_of(seq_ids)
-        ql = torch.tensor(counts, dtype=torch.int32, device=dev)
+        with self._undone(seq_ids, lens):
+            mgr.sync()
+            bt, sl, pages, shared = self._cache_of(seq_ids)
+            ql = torch.tensor(counts, dtype=torch.int32, device=dev)
 
-        def attend(q, pool):
-            q4 = torch.zeros(B * Q, self.H, self.hd, dtype=q.dtype, device=dev)
-            q4[at] = q
-            o = self.attn.forward_shared_prefix(q4.view(B, Q, self.H, self.hd), pool, bt, sl, pages, shared, ql)
-            return o.view(B * Q, self.H, self.hd)[at]
+            def attend(q, pool):
+                q4 = torch.zeros(B * Q, self.H, self.hd, dtype=q.dtype, device=dev)
+                q4[at] = q
+                o = self.attn.forward_shared_prefix(q4.view(B, Q, self.H, self.hd), pool, bt, sl, pages, shared, ql)
+                return o.view(B * Q, self.H, self.hd)[at]
 
-        lg = self._decode(toks, posn, rows, pos, attend)
-        if temperature > 0:
-            p = torch.softmax(lg / temperature, -1)
-        else:
-            p = torch.zeros_like(lg).scatter_(1, torch.argmax(lg, -1, keepdim=True), 1.0)
-        target = torch.zeros(B * Q, p.shape[1], device=dev)
-        target[at] = p
-        dt = torch.tensor([list(d) + [-1] * (Q - 1 - len(d)) for d in drafts], dtype=torch.long).view(B, Q - 1).to(dev)
-        if uniforms is None:
-            uniforms = torch.rand(B, Q, device=dev, generator=generator)
-        kept, new = verify_drafts(target.view(B, Q, -1), draft_probs, dt, uniforms,
-                                  torch.tensor([c - 1 for c in counts], dtype=torch.int32, device=dev))
-        out = [t[: k + 1] for k, t in zip(kept.tolist(), new.tolist())]
-        nothing = any(t[-1] < 0 for t in out)  # NaN logits: leave every sequence as it was
+            lg = self._decode(toks, posn, rows, pos, attend)
+            if temperature > 0:
+                p = torch.softmax(lg / temperature, -1)
+            else:
+                p = torch.zeros_like(lg).scatter_(1, torch.argmax(lg, -1, keepdim=True), 1.0)
+            target = torch.zeros(B * Q, p.shape[1], device=dev)
+            target[at] = p
+            dt = torch.tensor([list(d) + [-1] * (Q - 1 - len(d)) for d in drafts], dtype=torch.long)
+            if uniforms is None:
+                uniforms = torch.rand(B, Q, device=dev, generator=generator)
+            if draft_probs is not None:  # (a wider type holds the same values)
+                draft_probs = draft_probs.float()
+            kept, new = verify_drafts(target.view(B, Q, -1), draft_probs, dt.view(B, Q - 1).to(dev), uniforms,
+                                      torch.tensor([c - 1 for c in counts], dtype=torch.int32, device=dev))
+            out = [t[: k + 1] for k, t in zip(kept.tolist(), new.tolist())]
+            if any(t[-1] < 0 for t in out):  # NaN logits
+                raise InferenceError("the model's probabilities hold no token to draw")
         for s, a, t in zip(seq_ids, lens, out):
-            mgr.truncate_sequence(s, a if nothing else a + len(t))
-            if not nothing:
-                self.last_token[s] = t[-1]
-        if nothing:
-            raise InferenceError("the model's probabilities hold no token to draw")
+            mgr.truncate_sequence(s, a + len(t))
+            self.last_token[s] = t[-1]
         return out
 
     def generate(self, prompts: list[torch.Tensor], max_new_tokens: int, temperature: float = 0.0,

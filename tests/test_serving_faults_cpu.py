@@ -1,0 +1,74 @@
+"""Calls of the serving path that are refused or fail half way, samples at a temperature, logits and pages that are no
+numbers: what is left behind, and what comes out."""
+import pytest
+import torch
+
+from scirs_b200.inference import GPTGenerator, InferenceError
+from scirs_b200.models.gpt import GPTConfig, GPTModel
+
+V = 128
+
+
+def _generator(seqs=6):
+    m = GPTModel(GPTConfig.tiny(vocab=V, seq=64), device="cpu", seed=1)
+    return GPTGenerator(m, max_sequences=seqs, max_len=64, block_size=8)
+
+
+def _prompt(n=13):
+    return torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(3))
+
+
+# ------------------------------------------------------------------------------------------------ refused calls
+@pytest.mark.parametrize("bad", [
+    dict(draft_probs=torch.full((2, 2, V), 1.0 / V, dtype=torch.float64)),
+    dict(draft_probs=torch.ones(2, 2, V, dtype=torch.int64)),
+    dict(draft_probs=torch.empty(2, 2, V, device="meta")),
+    dict(uniforms=torch.rand(2, 3, dtype=torch.float64)),
+    dict(uniforms=torch.rand(2, 3).to(torch.bfloat16)),
+    dict(uniforms=torch.empty(2, 3, device="meta")),
+])
+def test_refused_verification_leaves_the_sequences(bad):
+    gen = _generator()
+    a = gen.add_sequence(_prompt())
+    b = gen.fork(a)
+    want = gen.step([a])[0], gen.step([a])[0]
+    gen.release(a)
+    free = gen.pools[0].free_count()
+    c = gen.fork(b)
+    with pytest.raises(InferenceError):
+        gen.verify([b, c], [[7, 9], [3]], **bad)
+    assert gen.manager.seq_len(b) == gen.manager.seq_len(c) == 13 and gen.pools[0].free_count() == free
+    assert (gen.step([b])[0], gen.step([b])[0]) == want
+
+
+def test_verification_that_fails_on_the_way_is_taken_back(monkeypatch):
+    gen = _generator()
+    a = gen.add_sequence(_prompt())
+    pending, chain = gen.last_token[a], gen.manager.sequence_page_chain(a)
+    want = gen.verify([a], [[7, 9, 11, 13]])
+    gen.manager.truncate_sequence(a, 13)
+    gen.last_token[a] = pending
+
+    def fails(*args):
+        raise RuntimeError("no memory")
+
+    for call in (lambda: gen.verify([a], [[7, 9, 11, 13]]), lambda: gen.step([a])):
+        with monkeypatch.context() as mp, pytest.raises(RuntimeError, match="no memory"):
+            mp.setattr(gen, "_decode", fails)
+            call()
+        assert gen.manager.seq_len(a) == 13 and gen.last_token[a] == pending
+        assert gen.manager.sequence_page_chain(a) == chain
+    assert gen.verify([a], [[7, 9, 11, 13]]) == want
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_draft_probabilities_of_sixteen_bits(dtype):
+    """They count as the values that they hold."""
+    q = torch.softmax(torch.randn(1, 3, V, generator=torch.Generator().manual_seed(1)), -1).to(dtype)
+    u = torch.tensor([[0.3, 0.9, 0.2, 0.6]])
+    out = []
+    for probs in (q, q.float()):
+        gen = _generator()
+        a = gen.add_sequence(_prompt())
+        out.append((gen.verify([a], [[5, 6, 7]], probs, temperature=1.0, uniforms=u), gen.manager.seq_len(a)))
+    assert out[0] == out[1]

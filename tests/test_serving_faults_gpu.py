@@ -1,0 +1,39 @@
+"""Serving operators on the GPU: calls that are refused, and places where a mistake would show only there."""
+import pytest
+import torch
+
+from scirs_b200 import _ext
+from scirs_b200.inference import GPTGenerator, InferenceError
+from scirs_b200.models.gpt import GPTConfig, GPTModel
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _generator(seqs=6, **kw):
+    m = GPTModel(GPTConfig.tiny(vocab=512, seq=256), device=DEV, seed=1)
+    return GPTGenerator(m, max_sequences=seqs, max_len=256, block_size=16, **kw)
+
+
+def _prompt(n=100):
+    return torch.randint(0, 512, (n,), generator=torch.Generator().manual_seed(3))
+
+
+# ------------------------------------------------------------------------------------------------ refused calls
+def test_refused_verification_leaves_the_sequences():
+    gen = _generator()
+    a = gen.add_sequence(_prompt())
+    b = gen.fork(a)
+    free = gen.pools[0].free_count()
+    want = [gen.step([b])[0] for _ in range(3)]
+    gen.release(b)
+    probs = torch.full((1, 2, 512), 1 / 512)
+    for bad in (dict(draft_probs=probs), dict(draft_probs=probs.double().to(DEV)), dict(uniforms=torch.rand(1, 3)),
+                dict(uniforms=torch.rand(1, 3, device=DEV).double())):
+        with pytest.raises(InferenceError):
+            gen.verify([a], [[7, 9]], **bad)
+        assert gen.manager.seq_len(a) == 100 and gen.pools[0].free_count() == free
+    assert [gen.step([a])[0] for _ in range(3)] == want
+    new = gen.verify([a], [[7, 9]], probs.to(DEV).to(torch.bfloat16), temperature=1.0)[0]
+    assert gen.manager.seq_len(a) == 103 + len(new)
+    _ext.check_status(0)
