@@ -72,10 +72,9 @@ class GPTGenerator:
                 self.manager.truncate_sequence(s, n)
             raise
 
-    # ----------------------------------------------------------- API
     @torch.no_grad()
-    def add_sequence(self, prompt: torch.Tensor) -> int:
-        """Prefill one prompt (1-D token tensor); returns the sequence id."""
+    def _prefill(self, prompt: torch.Tensor) -> tuple[int, torch.Tensor]:
+        """A new sequence with the prompt's tokens, without a pending one; its id and its last logits (fp32)."""
         m, H, hd = self.m, self.H, self.hd
         S = int(prompt.numel())
         assert 0 < S < self.max_len
@@ -90,8 +89,15 @@ class GPTGenerator:
         for l in range(self.L):
             qkv = A.qkv[l].view(S, 3, H, hd)
             self._append(l, rows, pos, qkv[:, 1], qkv[:, 2])
-        nxt = int(torch.argmax(logits[0, -1].float()))
-        self.last_token[sid] = nxt
+        return sid, logits[0, -1].float()
+
+    # ----------------------------------------------------------- API
+    @torch.no_grad()
+    def add_sequence(self, prompt: torch.Tensor) -> int:
+        """Prefill one prompt (1-D token tensor); returns the sequence id. The model's own choice (the
+        largest logit) is the sequence's pending token."""
+        sid, logits = self._prefill(prompt)
+        self.last_token[sid] = int(torch.argmax(logits))
         return sid
 
     def fork(self, seq_id: int) -> int:
@@ -250,13 +256,22 @@ class GPTGenerator:
     def generate(self, prompts: list[torch.Tensor], max_new_tokens: int, temperature: float = 0.0,
                  num_samples: int = 1) -> list[list[int]]:
         """Greedy (temperature 0) or sampled continuation of every prompt, num_samples of each (prompt
-        by prompt; the prompt is processed once and forked)."""
+        by prompt; the prompt is processed once and forked). At a temperature every token of every
+        sample is drawn, the first one too."""
         if num_samples < 1:
             raise ValueError("num_samples must be at least 1")
         ids = []
         for p in prompts:
-            ids.append(self.add_sequence(p))
-            ids += [self.fork(ids[-1]) for _ in range(num_samples - 1)]
+            sid, logits = self._prefill(p)
+            if temperature > 0:
+                first = torch.multinomial(torch.softmax(logits / temperature, -1), num_samples, replacement=True).tolist()
+            else:
+                first = [int(torch.argmax(logits))] * num_samples
+            self.last_token[sid] = first[0]
+            ids.append(sid)
+            for t in first[1:]:
+                ids.append(self.fork(sid))
+                self.last_token[ids[-1]] = t
         outs = {s: [self.last_token[s]] for s in ids}
         for _ in range(max_new_tokens - 1):
             for s, t in zip(ids, self.step(ids, temperature)):

@@ -72,3 +72,32 @@ def test_draft_probabilities_of_sixteen_bits(dtype):
         a = gen.add_sequence(_prompt())
         out.append((gen.verify([a], [[5, 6, 7]], probs, temperature=1.0, uniforms=u), gen.manager.seq_len(a)))
     assert out[0] == out[1]
+
+
+# ------------------------------------------------------------------------------------------------ samples
+@pytest.mark.parametrize("groups", [1, 8])
+def test_first_tokens_of_samples_follow_the_distribution(groups):
+    """N first tokens at a temperature, all of one prompt and in several calls."""
+    N, T = 1600, 0.7
+    gen = _generator(seqs=N // groups)
+    gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], logits))(gen._prefill)
+    logits = torch.full((V,), float("-inf"))
+    logits[[3, 50, 77, 127]] = torch.tensor([0.5, 0.25, 0.125, 0.125]).log() * T
+    torch.manual_seed(7)
+    first = []
+    for _ in range(groups):
+        first += [o[0] for o in gen.generate([_prompt(3)], 1, temperature=T, num_samples=N // groups)]
+    assert len(first) == N
+    emp = torch.bincount(torch.tensor(first), minlength=V) / N
+    p = torch.softmax(logits, -1)
+    # 5 standard deviations of a frequency: 5 sqrt(p (1 - p) / N) <= 5 * 0.5 / 40
+    assert (emp - p).abs().max() < 0.0625 and emp[p == 0].sum() == 0
+
+
+def test_samples_at_a_high_temperature_begin_differently():
+    gen = _generator()
+    torch.manual_seed(0)
+    # the model's distribution at temperature 50 is near to uniform over 128: six equal first tokens have odds of 128^-5
+    assert len({o[0] for o in gen.generate([_prompt()], 3, temperature=50.0, num_samples=6)}) > 1
+    assert len({gen.generate([_prompt()], 2, temperature=50.0)[0][0] for _ in range(6)}) > 1
+    assert gen.pools[0].free_count() == gen.pools[0].total_count()
