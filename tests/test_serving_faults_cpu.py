@@ -89,7 +89,7 @@ def test_first_tokens_of_samples_follow_the_distribution(groups):
         first += [o[0] for o in gen.generate([_prompt(3)], 1, temperature=T, num_samples=N // groups)]
     assert len(first) == N
     emp = torch.bincount(torch.tensor(first), minlength=V) / N
-    p = torch.softmax(logits, -1)
+    p = torch.softmax(logits / T, -1)
     # 5 standard deviations of a frequency: 5 sqrt(p (1 - p) / N) <= 5 * 0.5 / 40
     assert (emp - p).abs().max() < 0.0625 and emp[p == 0].sum() == 0
 
