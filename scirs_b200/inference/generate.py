@@ -264,7 +264,9 @@ class GPTGenerator:
         for p in prompts:
             sid, logits = self._prefill(p)
             if temperature > 0:
-                first = torch.multinomial(torch.softmax(logits / temperature, -1), num_samples, replacement=True).tolist()
+                # (a row each: draws of one row with replacement would check it by an assertion on the device)
+                probs = torch.softmax(logits / temperature, -1).expand(num_samples, -1)
+                first = torch.multinomial(probs, 1).view(-1).tolist()
             else:
                 first = [int(torch.argmax(logits))] * num_samples
             self.last_token[sid] = first[0]

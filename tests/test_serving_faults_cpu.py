@@ -101,3 +101,10 @@ def test_samples_at_a_high_temperature_begin_differently():
     assert len({o[0] for o in gen.generate([_prompt()], 3, temperature=50.0, num_samples=6)}) > 1
     assert len({gen.generate([_prompt()], 2, temperature=50.0)[0][0] for _ in range(6)}) > 1
     assert gen.pools[0].free_count() == gen.pools[0].total_count()
+
+
+def test_samples_of_logits_that_are_no_numbers_are_refused():
+    gen = _generator()
+    gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], torch.full((V,), float("nan"))))(gen._prefill)
+    with pytest.raises(RuntimeError):
+        gen.generate([_prompt()], 2, temperature=1.0, num_samples=3)

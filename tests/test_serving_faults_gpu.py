@@ -37,3 +37,23 @@ def test_refused_verification_leaves_the_sequences():
     new = gen.verify([a], [[7, 9]], probs.to(DEV).to(torch.bfloat16), temperature=1.0)[0]
     assert gen.manager.seq_len(a) == 103 + len(new)
     _ext.check_status(0)
+
+
+# ------------------------------------------------------------------------------------------------ samples
+def test_samples_of_logits_that_are_no_numbers_are_refused():
+    gen = _generator()
+    nan = torch.full((512,), float("nan"), device=DEV)
+    gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], nan))(gen._prefill)
+    with pytest.raises(RuntimeError):
+        gen.generate([_prompt()], 2, temperature=1.0, num_samples=3)
+    torch.cuda.synchronize()  # (the error was the host's: the device goes on)
+    assert float(nan.nan_to_num(1.0).sum()) == 512.0
+
+
+def test_samples_begin_differently():
+    gen = _generator()
+    torch.manual_seed(0)
+    # near to uniform over 512 tokens at temperature 50: six equal first tokens have odds of 512^-5
+    assert len({o[0] for o in gen.generate([_prompt(), _prompt(20)], 3, temperature=50.0, num_samples=3)}) > 1
+    assert gen.pools[0].free_count() == gen.pools[0].total_count()
+    _ext.check_status(0)
