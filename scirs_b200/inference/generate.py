@@ -235,7 +235,8 @@ class GPTGenerator:
             if temperature > 0:
                 p = torch.softmax(lg / temperature, -1)
             else:
-                p = torch.zeros_like(lg).scatter_(1, torch.argmax(lg, -1, keepdim=True), 1.0)
+                best = torch.argmax(lg, -1, keepdim=True)  # (a NaN, where the row holds one: no token then)
+                p = torch.zeros_like(lg).scatter_(1, best, 1.0 - torch.isnan(lg.gather(1, best)).float())
             target = torch.zeros(B * Q, p.shape[1], device=dev)
             target[at] = p
             dt = torch.tensor([list(d) + [-1] * (Q - 1 - len(d)) for d in drafts], dtype=torch.long)
@@ -246,7 +247,7 @@ class GPTGenerator:
             kept, new = verify_drafts(target.view(B, Q, -1), draft_probs, dt.view(B, Q - 1).to(dev), uniforms,
                                       torch.tensor([c - 1 for c in counts], dtype=torch.int32, device=dev))
             out = [t[: k + 1] for k, t in zip(kept.tolist(), new.tolist())]
-            if any(t[-1] < 0 for t in out):  # NaN logits
+            if any(t[-1] < 0 for t in out):  # logits that are no numbers
                 raise InferenceError("the model's probabilities hold no token to draw")
         for s, a, t in zip(seq_ids, lens, out):
             mgr.truncate_sequence(s, a + len(t))

@@ -108,3 +108,33 @@ def test_samples_of_logits_that_are_no_numbers_are_refused():
     gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], torch.full((V,), float("nan"))))(gen._prefill)
     with pytest.raises(RuntimeError):
         gen.generate([_prompt()], 2, temperature=1.0, num_samples=3)
+
+
+# ------------------------------------------------------------------------------------------------ numbers that are none
+@pytest.mark.parametrize("temperature,row", [(0.0, 0), (0.0, 1), (0.0, None), (1.0, 0), (1.0, None)])
+def test_verification_of_logits_that_are_no_numbers(temperature, row):
+    """Row 0 belongs to the pending token, row 1 to the draft (refused where it is not the model's choice)."""
+    gen = _generator()
+    a = gen.add_sequence(_prompt())
+    size, pending, decode = gen.manager.seq_len(a), gen.last_token[a], gen._decode
+
+    def nan(*args):
+        lg = decode(*args)
+        lg[slice(None) if row is None else row, 5] = float("nan")
+        return lg
+
+    best = gen.step([a])[0]
+    gen.manager.truncate_sequence(a, size)
+    gen.last_token[a] = pending
+    gen._decode = nan
+    uniforms = torch.full((1, 2), 0.5)
+    if row == 1 and temperature == 0.0:  # a refused draft: its row is not looked at
+        assert gen.verify([a], [[(best + 1) % 100]], temperature=temperature, uniforms=uniforms) == [[best]]
+        gen.manager.truncate_sequence(a, size)
+        gen.last_token[a] = pending
+    draft = [best] if temperature == 0.0 else []
+    with pytest.raises(InferenceError, match="no token"):
+        gen.verify([a], [draft], temperature=temperature, uniforms=uniforms[:, : 1 + len(draft)])
+    assert gen.manager.seq_len(a) == size and gen.last_token[a] == pending
+    gen._decode = decode
+    assert gen.step([a]) == [best]

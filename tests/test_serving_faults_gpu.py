@@ -57,3 +57,33 @@ def test_samples_begin_differently():
     assert len({o[0] for o in gen.generate([_prompt(), _prompt(20)], 3, temperature=50.0, num_samples=3)}) > 1
     assert gen.pools[0].free_count() == gen.pools[0].total_count()
     _ext.check_status(0)
+
+
+# ------------------------------------------------------------------------------------------------ numbers that are none
+@pytest.mark.parametrize("temperature,row", [(0.0, 0), (0.0, 1), (0.0, None), (1.0, 0), (1.0, None)])
+def test_verification_of_logits_that_are_no_numbers(temperature, row):
+    """Row 0 belongs to the pending token, row 1 to the draft (refused where it is not the model's choice)."""
+    gen = _generator()
+    a = gen.add_sequence(_prompt())
+    size, pending, decode = gen.manager.seq_len(a), gen.last_token[a], gen._decode
+
+    def nan(*args):
+        lg = decode(*args)
+        lg[slice(None) if row is None else row, 5] = float("nan")
+        return lg
+
+    best = gen.step([a])[0]
+    gen.manager.truncate_sequence(a, size)
+    gen.last_token[a] = pending
+    gen._decode = nan
+    uniforms = torch.full((1, 2), 0.5, device=DEV)
+    if row == 1 and temperature == 0.0:  # a refused draft: its row is not looked at
+        assert gen.verify([a], [[(best + 1) % 100]], temperature=temperature, uniforms=uniforms) == [[best]]
+        gen.manager.truncate_sequence(a, size)
+        gen.last_token[a] = pending
+    draft = [best] if temperature == 0.0 else []
+    with pytest.raises(InferenceError, match="no token"):
+        gen.verify([a], [draft], temperature=temperature, uniforms=uniforms[:, : 1 + len(draft)])
+    assert gen.manager.seq_len(a) == size and gen.last_token[a] == pending
+    gen._decode = decode
+    assert gen.step([a]) == [best]
