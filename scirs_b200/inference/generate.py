@@ -81,14 +81,18 @@ class GPTGenerator:
         sid = self._next_id
         self._next_id += 1
         self.manager.allocate_sequence(sid)
-        rows, pos = self.manager.reserve([sid], [S])
-        self.manager.sync()
-        tok = prompt.to(m.device).reshape(1, S)
-        logits = m.logits(tok)  # runs every layer; keeps qkv per layer in the activations
-        A = m._acts
-        for l in range(self.L):
-            qkv = A.qkv[l].view(S, 3, H, hd)
-            self._append(l, rows, pos, qkv[:, 1], qkv[:, 2])
+        try:
+            rows, pos = self.manager.reserve([sid], [S])
+            self.manager.sync()
+            tok = prompt.to(m.device).reshape(1, S)
+            logits = m.logits(tok)  # runs every layer; keeps qkv per layer in the activations
+            A = m._acts
+            for l in range(self.L):
+                qkv = A.qkv[l].view(S, 3, H, hd)
+                self._append(l, rows, pos, qkv[:, 1], qkv[:, 2])
+        except BaseException:  # no pages for the prompt, say: no half-made sequence stays behind
+            self.manager.free_sequence(sid)
+            raise
         return sid, logits[0, -1].float()
 
     # ----------------------------------------------------------- API
@@ -262,25 +266,27 @@ class GPTGenerator:
         if num_samples < 1:
             raise ValueError("num_samples must be at least 1")
         ids = []
-        for p in prompts:
-            sid, logits = self._prefill(p)
-            if temperature > 0:
-                # (a row each: draws of one row with replacement would check it by an assertion on the device)
-                probs = torch.softmax(logits / temperature, -1).expand(num_samples, -1)
-                first = torch.multinomial(probs, 1).view(-1).tolist()
-            else:
-                first = [int(torch.argmax(logits))] * num_samples
-            self.last_token[sid] = first[0]
-            ids.append(sid)
-            for t in first[1:]:
-                ids.append(self.fork(sid))
-                self.last_token[ids[-1]] = t
-        outs = {s: [self.last_token[s]] for s in ids}
-        for _ in range(max_new_tokens - 1):
-            for s, t in zip(ids, self.step(ids, temperature)):
-                outs[s].append(t)
-        for s in ids:
-            self.release(s)
+        try:
+            for p in prompts:
+                sid, logits = self._prefill(p)
+                ids.append(sid)
+                if temperature > 0:
+                    # (a row each: draws of one row with replacement would check it by an assertion on the device)
+                    probs = torch.softmax(logits / temperature, -1).expand(num_samples, -1)
+                    first = torch.multinomial(probs, 1).view(-1).tolist()
+                else:
+                    first = [int(torch.argmax(logits))] * num_samples
+                self.last_token[sid] = first[0]
+                for t in first[1:]:
+                    ids.append(self.fork(sid))
+                    self.last_token[ids[-1]] = t
+            outs = {s: [self.last_token[s]] for s in ids}
+            for _ in range(max_new_tokens - 1):
+                for s, t in zip(ids, self.step(ids, temperature)):
+                    outs[s].append(t)
+        finally:  # no row or page left for a sample, say: those that were made are given back
+            for s in ids:
+                self.release(s)
         return [outs[s] for s in ids]
 
     def release(self, seq_id: int):

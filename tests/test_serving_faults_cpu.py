@@ -138,3 +138,35 @@ def test_verification_of_logits_that_are_no_numbers(temperature, row):
     assert gen.manager.seq_len(a) == size and gen.last_token[a] == pending
     gen._decode = decode
     assert gen.step([a]) == [best]
+
+
+# ------------------------------------------------------------------------------------------------ nothing left behind
+def test_generation_that_finds_no_room_leaves_nothing_behind():
+    gen = _generator(seqs=3)
+    total = gen.pools[0].total_count()
+
+    def empty():
+        return (gen.manager.active_sequences() == 0 and gen.pools[0].free_count() == total and not gen.last_token
+                and len(gen.manager._free_rows) == 3)
+
+    with pytest.raises(InferenceError, match="too many"):
+        gen.generate([_prompt()], 4, num_samples=4)
+    assert empty()
+    with pytest.raises(InferenceError, match="too many"):
+        gen.generate([_prompt(), _prompt(5)], 4, temperature=1.0, num_samples=2)
+    assert empty()
+    # pages: two prompts fit, their third sequence finds none
+    held = [gen.pools[0].alloc_page() for _ in range(total - 4)]
+    total = 4
+    with pytest.raises(InferenceError, match="exhausted"):
+        gen.generate([_prompt(13), _prompt(13), _prompt(13)], 4)
+    assert empty()
+    with pytest.raises(InferenceError, match="exhausted"):  # the prompt's second page is not there
+        gen.pools[0].retain_page(held[0])
+        extra = [gen.pools[0].alloc_page() for _ in range(3)]
+        gen.add_sequence(_prompt(13))
+    total = 1
+    assert empty()
+    for p in extra:
+        gen.pools[0].free_page(p)
+    assert len(gen.generate([_prompt()], 4, num_samples=2)) == 2
