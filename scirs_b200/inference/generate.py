@@ -201,6 +201,8 @@ class GPTGenerator:
             raise InferenceError("one list of drafts per sequence")
         if len(set(seq_ids)) < B:
             raise InferenceError("a sequence is verified once at a time")
+        if not B:
+            return []
         counts = [1 + len(d) for d in drafts]
         Q = max(counts)
         lens = [mgr.seq_len(s) for s in seq_ids]

@@ -74,6 +74,13 @@ def test_draft_probabilities_of_sixteen_bits(dtype):
     assert out[0] == out[1]
 
 
+def test_verification_of_no_sequences():
+    gen = _generator()
+    assert gen.verify([], []) == []
+    with pytest.raises(InferenceError):
+        gen.verify([], [[1]])
+
+
 # ------------------------------------------------------------------------------------------------ samples
 @pytest.mark.parametrize("groups", [1, 8])
 def test_first_tokens_of_samples_follow_the_distribution(groups):
