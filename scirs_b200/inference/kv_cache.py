@@ -265,7 +265,8 @@ class BlockManager:
 
     def compact(self) -> dict[int, int]:
         """Move the chains' pages to the front of the pool, into the free pages there, and return
-        {old page: new page}. Pages that something else holds too (retain_page, alloc_page) stay."""
+        {old page: new page}. Pages that something else holds too (retain_page, alloc_page, a
+        SharedPrefixCache with the pool) stay."""
         pool = self.pool
         held: dict[int, int] = {}
         for pages in self._pages.values():
@@ -406,19 +407,38 @@ class BlockManager:
 
 class SharedPrefixCache:
     """Maps a prompt-prefix hash to the page chain that holds its K/V, so
-    sequences with a common prompt can reuse the pages."""
+    sequences with a common prompt can reuse the pages.
 
-    def __init__(self):
+    With the chains' `pool` the cache holds every page that it lists (insert
+    retains it, evict gives it back): a listed page is not reused when its
+    sequences end, not written by the ones that go on, and not moved by
+    BlockManager.compact. Without one it keeps page ids alone, which those
+    calls make stale."""
+
+    def __init__(self, pool: KvPagePool | None = None):
+        self._pool = pool
         self._map: dict[int, list[int]] = {}
 
     def lookup(self, prefix_hash: int):
         return self._map.get(prefix_hash)
 
     def insert(self, prefix_hash: int, pages: list[int]) -> None:
-        self._map[prefix_hash] = list(pages)
+        pages = list(pages)
+        if self._pool is not None:
+            for pid in pages:
+                if self._pool.ref_count(pid) == 0:
+                    raise InferenceError(f"page {pid} is not allocated")
+            for pid in pages:
+                self._pool.retain_page(pid)
+        self.evict(prefix_hash)
+        self._map[prefix_hash] = pages
 
     def evict(self, prefix_hash: int):
-        return self._map.pop(prefix_hash, None)
+        pages = self._map.pop(prefix_hash, None)
+        if self._pool is not None:
+            for pid in pages or ():
+                self._pool.free_page(pid)
+        return pages
 
     def __len__(self):
         return len(self._map)

@@ -3,7 +3,8 @@ numbers: what is left behind, and what comes out."""
 import pytest
 import torch
 
-from scirs_b200.inference import GPTGenerator, InferenceError
+from scirs_b200.inference import (BlockManager, BlockManagerConfig, GPTGenerator, InferenceError, KvPageConfig,
+                                  KvPagePool, SharedPrefixCache)
 from scirs_b200.models.gpt import GPTConfig, GPTModel
 
 V = 128
@@ -177,3 +178,38 @@ def test_generation_that_finds_no_room_leaves_nothing_behind():
     for p in extra:
         gen.pools[0].free_page(p)
     assert len(gen.generate([_prompt()], 4, num_samples=2)) == 2
+
+
+# ------------------------------------------------------------------------------------------------ cached prefixes
+def test_pages_of_a_prefix_cache_stay():
+    pool = KvPagePool(8, KvPageConfig(block_size=4, num_heads=2, head_dim=8), "cpu")
+    bm = BlockManager(pool, BlockManagerConfig(4, 8))
+    cache = SharedPrefixCache(pool)
+
+    def write(seq, n, value):
+        kv = torch.full((n, 2, 8), value).to(torch.bfloat16)
+        bm.append([seq], [n], kv, -kv)
+
+    bm.allocate_sequence(0)
+    write(0, 4, 1.0)
+    bm.allocate_sequence(1)
+    write(1, 8, 2.0)
+    cache.insert(5, bm.sequence_page_chain(1))
+    listed = list(cache.lookup(5))
+    bm.fork_sequence(1, 2)
+    bm.free_sequence(0)  # a hole in front of the listed pages
+    write(2, 4, 3.0)
+    moves = bm.compact()
+    assert moves and cache.lookup(5) == listed == bm.sequence_page_chain(1)[:2] == bm.sequence_page_chain(2)[:2]
+    bm.free_sequence(1)
+    bm.free_sequence(2)
+    assert [pool.ref_count(p) for p in listed] == [1, 1] and pool.free_count() == 6
+    assert (pool.k[listed] == 2.0).all() and (pool.v[listed] == -2.0).all()
+    # a refused entry changes nothing, another chain under the hash takes the place of the first, which is given back
+    free = next(p for p in range(8) if pool.ref_count(p) == 0)
+    with pytest.raises(InferenceError):
+        cache.insert(5, [listed[0], free])
+    assert cache.lookup(5) == listed and pool.ref_count(listed[0]) == 1
+    cache.insert(5, listed[:1])
+    assert [pool.ref_count(p) for p in listed] == [1, 0]
+    assert cache.evict(5) == listed[:1] and cache.evict(5) is None and pool.free_count() == 8
