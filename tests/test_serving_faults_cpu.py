@@ -197,8 +197,8 @@ def test_pages_of_a_prefix_cache_stay():
     cache.insert(5, bm.sequence_page_chain(1))
     listed = list(cache.lookup(5))
     bm.fork_sequence(1, 2)
-    bm.free_sequence(0)  # a hole in front of the listed pages
     write(2, 4, 3.0)
+    bm.free_sequence(0)  # a hole in front of the listed pages
     moves = bm.compact()
     assert moves and cache.lookup(5) == listed == bm.sequence_page_chain(1)[:2] == bm.sequence_page_chain(2)[:2]
     bm.free_sequence(1)
