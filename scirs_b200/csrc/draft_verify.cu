@@ -249,7 +249,8 @@ std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10:
   CHECK_CUDA_TENSOR(target);
   TORCH_CHECK(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1, "target probabilities [B, n + 1, V]");
   const int64_t B = target.size(0), n = target.size(1) - 1, V = target.size(2);
-  TORCH_CHECK(V < (1LL << 31) - 64 && B < 65536 && n < (1LL << 31), "draft_verify: too large");
+  // (places in a row are 32-bit numbers; the end of the last segment lies up to a segment behind the row's)
+  TORCH_CHECK(V < (1LL << 30) && B < 65536 && n < (1LL << 30), "draft_verify: too large");
   auto rows = [&](const torch::Tensor& t, const char* what, int64_t count) {
     TORCH_CHECK(t.device() == target.device() && t.scalar_type() == target.scalar_type() && t.dim() == 3 &&
                     t.size(0) == B && t.size(1) == count && t.size(2) == V && (V == 1 || t.stride(2) == 1),

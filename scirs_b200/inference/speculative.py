@@ -132,11 +132,14 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, 
     not kept one token is drawn from max(p - q, 0), or from p where that is zero everywhere, and from
     the last p where all are kept: the first token whose cumulative weight exceeds u_n times the
     total. The weights need not sum to 1; negative, infinite and NaN ones count as zero, and -1 is
-    returned in the token's place where nothing is left. Products and sums are formed in 64 bits."""
+    returned in the token's place where nothing is left. Products and sums are formed in 64 bits.
+    V and n are below 2^30."""
     t, d = target_probs, draft_probs
     if t.dim() != 3 or t.shape[1] < 1 or t.shape[2] < 1:
         raise ValueError("target probabilities must be [B, n + 1, V]")
     B, n, V = t.shape[0], t.shape[1] - 1, t.shape[2]
+    if V >= 1 << 30 or n >= 1 << 30:
+        raise ValueError("fewer than 2^30 tokens and drafts")
     if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError("probabilities must be fp32, bf16 or fp16")
     if d is not None and (d.shape != (B, n, V) or d.dtype != t.dtype or d.device != t.device):

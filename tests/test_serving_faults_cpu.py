@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from scirs_b200.inference import (BlockManager, BlockManagerConfig, GPTGenerator, InferenceError, KvPageConfig,
-                                  KvPagePool, SharedPrefixCache)
+                                  KvPagePool, SharedPrefixCache, verify_drafts)
 from scirs_b200.models.gpt import GPTConfig, GPTModel
 
 V = 128
@@ -213,3 +213,13 @@ def test_pages_of_a_prefix_cache_stay():
     cache.insert(5, listed[:1])
     assert [pool.ref_count(p) for p in listed] == [1, 0]
     assert cache.evict(5) == listed[:1] and cache.evict(5) is None and pool.free_count() == 8
+
+
+# ------------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("n,vocab", [(1, 1 << 30), (1, (1 << 31) - 65), (1 << 30, 1)])
+def test_verification_refuses_rows_of_more_than_thirty_bits(n, vocab):
+    def like(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    with pytest.raises(ValueError, match="2\\^30"):
+        verify_drafts(like(1, n + 1, vocab), like(1, n, vocab), like(1, n, dtype=torch.int64), like(1, n + 1))
