@@ -87,11 +87,12 @@ void paged_kv_append(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor k_p
 void paged_attention_decode(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor block_tables,
                             torch::Tensor seq_lens, torch::Tensor out, torch::Tensor part_o, torch::Tensor part_ml,
                             int64_t tokens_per_split, double scale);
-torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
-                                     torch::Tensor lens, torch::Tensor pages, int64_t L,
-                                     c10::optional<torch::Tensor> qlens, double scale);
-void page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor dst,
-               c10::optional<torch::Tensor> counts);
+std::tuple<torch::Tensor, int64_t> paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                                          torch::Tensor tables, torch::Tensor lens,
+                                                          torch::Tensor pages, int64_t L,
+                                                          c10::optional<torch::Tensor> qlens, double scale);
+int64_t page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor dst,
+                  c10::optional<torch::Tensor> counts);
 std::tuple<torch::Tensor, torch::Tensor> draft_verify(torch::Tensor target, c10::optional<torch::Tensor> draft,
                                                       torch::Tensor tokens, torch::Tensor uniforms,
                                                       c10::optional<torch::Tensor> lens, double threshold);
@@ -166,8 +167,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_kv_append", &scirs::paged_kv_append);
   m.def("paged_attention_decode", &scirs::paged_attention_decode);
   m.def("paged_prefix_attention", &scirs::paged_prefix_attention,
-        "attention over the paged cache for a batch that shares a prefix");
-  m.def("page_copy", &scirs::page_copy, "copy pages of every layer's pools");
+        "attention over the paged cache for a batch that shares a prefix: (output, launches)");
+  m.def("page_copy", &scirs::page_copy, "copy pages of every layer's pools; returns the launches");
   m.def("draft_verify", &scirs::draft_verify, "keep or replace drafted tokens");
   m.def("flash_attn_fwd_pp", &scirs::flash_attn_fwd_pp, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
         py::arg("lse"), py::arg("causal"), py::arg("scale"), py::arg("poly") = false,

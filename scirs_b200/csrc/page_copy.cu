@@ -48,13 +48,15 @@ __global__ void __launch_bounds__(kThreads) copy_kernel(const __grid_constant__ 
   }
 }
 
+// Returns how many launches it took.
 template <int MOVES, int BUFS, int U>
-void launch(const std::vector<torch::Tensor>& bufs, const int* src, const int* dst, const int* counts, int n,
+int64_t launch(const std::vector<torch::Tensor>& bufs, const int* src, const int* dst, const int* counts, int n,
             int slot_vecs, int block_size) {
   const int dev = bufs[0].get_device();
   Args<MOVES, BUFS> a;
   a.page_vecs = (long)slot_vecs * block_size;
   a.chunks = (int)((a.page_vecs + kThreads * U - 1) / (kThreads * U));
+  int64_t launches = 0;
   for (size_t b0 = 0; b0 < bufs.size(); b0 += BUFS) {
     a.bufs = (int)std::min<size_t>(BUFS, bufs.size() - b0);
     for (int b = 0; b < a.bufs; ++b) a.buf[b] = reinterpret_cast<uint4*>(bufs[b0 + b].data_ptr());
@@ -69,16 +71,18 @@ void launch(const std::vector<torch::Tensor>& bufs, const int* src, const int* d
       const int grid = (int)std::min<long>(units, 8L * num_sms(dev));
       copy_kernel<MOVES, BUFS, U><<<grid, kThreads, 0, cur_stream()>>>(a);
       SCIRS_CHECK_LAUNCH();
+      ++launches;
     }
   }
+  return launches;
 }
 
 }  // namespace pages
 
 // bufs: the pools ([num_pages, block_size, Hkv, HD], all of one shape and type on one device);
-// src / dst / counts: int32 on the host. Every index is checked here, before the launch.
-void page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor dst,
-               c10::optional<torch::Tensor> counts) {
+// src / dst / counts: int32 on the host. Every index is checked here, before the launch. Returns the launches made.
+int64_t page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor dst,
+                  c10::optional<torch::Tensor> counts) {
   TORCH_CHECK(!bufs.empty(), "page_copy: no pools");
   const torch::Tensor& f = bufs[0];
   TORCH_CHECK(f.is_cuda() && f.dim() == 4, "pools: CUDA [num_pages, block_size, Hkv, HD]");
@@ -108,9 +112,9 @@ void page_copy(std::vector<torch::Tensor> bufs, torch::Tensor src, torch::Tensor
     written[d[i]] = 1;
   }
   for (int64_t i = 0; i < n; ++i) TORCH_CHECK(!written[s[i]], "page ", num(s[i]), " is both read and written");
-  if (n == 0) return;
+  if (n == 0) return 0;
   c10::cuda::CUDAGuard guard(f.get_device());
-  pages::launch<1024, 256, 4>(bufs, s, d, c, (int)n, (int)(slot_bytes / 16), (int)bs);
+  return pages::launch<1024, 256, 4>(bufs, s, d, c, (int)n, (int)(slot_bytes / 16), (int)bs);
 }
 
 }  // namespace scirs

@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 
 }  // namespace prefix
 
-// q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape. Pools [num_pages, block_size,
+// q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape, and the launches made. Pools [num_pages, block_size,
 // Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
 // [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
 // tcgen05 takes the prefix from kTcKeys keys on if more than kTcRows rows share a cached head, and from kTcLong
@@ -590,9 +590,10 @@ constexpr int64_t kMinKeys = 128, kParts = 32;
 // Up to here a warp joins a row's parts, above four do (2048 rows of 20 parts: 9 us with four).
 constexpr int kFewParts = 8;
 
-torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor tables,
-                                     torch::Tensor lens, torch::Tensor pages, int64_t L,
-                                     c10::optional<torch::Tensor> qlens, double scale) {
+std::tuple<torch::Tensor, int64_t> paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                                          torch::Tensor tables, torch::Tensor lens,
+                                                          torch::Tensor pages, int64_t L,
+                                                          c10::optional<torch::Tensor> qlens, double scale) {
   CHECK_CUDA_TENSOR(q);
   CHECK_DTYPE(q, at::kBFloat16);
   CHECK_DTYPE(k_pool, at::kBFloat16);
@@ -630,7 +631,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
   TORCH_CHECK(max_pages * bs < (1LL << 30) && B * Q * H < (1LL << 30), "paged attention: too large");
   c10::cuda::CUDAGuard guard(q.get_device());
   auto out = at::empty(shape, q.options());
-  if (out.numel() == 0) return out;
+  if (out.numel() == 0) return {out, 0};
   if (q.stride(3) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || q.stride(2) % 8 ||
       reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
     q = q.clone(at::MemoryFormat::Contiguous);  // (contiguous() would keep a contiguous tensor at an odd offset)
@@ -733,7 +734,7 @@ torch::Tensor paged_prefix_attention(torch::Tensor q, torch::Tensor k_pool, torc
     prefix::launch(prefix::combine_kernel<4>, (unsigned)(B * Q * H), 128, 0, st, true, p);
   else
     prefix::launch(prefix::combine_kernel<1>, (unsigned)((B * Q * H + 3) / 4), 128, 0, st, true, p);
-  return out;
+  return {out, tc ? 3 : 2};
 }
 
 }  // namespace scirs

@@ -133,7 +133,8 @@ class KvPagePool:
 
 def copy_pages(pools, src, dst, counts=None) -> None:
     """Copy page ``src[i]`` to page ``dst[i]`` in each of ``pools`` (a :class:`KvPagePool` or a
-    list of alike ones, such as the layers'), keys and values, in one launch on the current stream.
+    list of alike ones, such as the layers'), keys and values, on the current stream: in one launch,
+    as far as there are up to 128 pools and 1024 pages.
 
     ``src``, ``dst`` and ``counts`` are lists or int32 host tensors; ``counts[i]`` limits the copy
     to the first so many slots of a page (default: all of them), the others keep what they hold.
@@ -148,8 +149,7 @@ def copy_pages(pools, src, dst, counts=None) -> None:
                         for t in (src, dst, counts))
     bufs = [b for p in pools for b in (p.k, p.v)]
     if bufs[0].is_cuda:
-        _ext.kernels().page_copy(bufs, src, dst, counts)
-        K._count(1)
+        K._count(_ext.kernels().page_copy(bufs, src, dst, counts))
         return
     for t in (src, dst, counts):
         if t is not None and (t.is_cuda or t.dtype != torch.int32 or t.shape != (src.numel(),)):

@@ -103,9 +103,9 @@ class PagedAttentionForward:
         if q.is_cuda:
             if q.dtype != torch.bfloat16:
                 q = q.to(torch.bfloat16)
-            out = _ext.kernels().paged_prefix_attention(q, pool.k, pool.v, block_tables, seq_lens, prefix_pages,
-                                                        int(prefix_len), q_lens, scale)
-            K._count(2)
+            out, launches = _ext.kernels().paged_prefix_attention(q, pool.k, pool.v, block_tables, seq_lens,
+                                                                  prefix_pages, int(prefix_len), q_lens, scale)
+            K._count(launches)
             return out
         q4 = q.unsqueeze(1) if q.dim() == 3 else q
         out = shared_prefix_attention_reference(q4, pool, block_tables, seq_lens, prefix_pages, prefix_len, q_lens,

@@ -157,7 +157,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_probs: torch.Tensor | None, 
         out = _ext.kernels().draft_verify(t, d, draft_tokens.contiguous(), uniforms.contiguous(),
                                           None if draft_lens is None else draft_lens.contiguous(),
                                           float(acceptance_threshold))
-        K._count(1)
+        K._count(1 if B else 0)
         return DraftVerification(*out)
     accepted, tokens = torch.zeros(B, dtype=torch.int32), torch.full((B, n + 1), -1, dtype=torch.int64)
     for b in range(B):

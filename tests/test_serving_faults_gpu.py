@@ -3,8 +3,10 @@ import pytest
 import torch
 
 from scirs_b200 import _ext
-from scirs_b200.inference import GPTGenerator, InferenceError
+from scirs_b200.inference import (GPTGenerator, InferenceError, KvPageConfig, KvPagePool, PagedAttentionConfig,
+                                  PagedAttentionForward, copy_pages, verify_drafts)
 from scirs_b200.models.gpt import GPTConfig, GPTModel
+from scirs_b200.ops import kernels as K
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -87,3 +89,32 @@ def test_verification_of_logits_that_are_no_numbers(temperature, row):
     assert gen.manager.seq_len(a) == size and gen.last_token[a] == pending
     gen._decode = decode
     assert gen.step([a]) == [best]
+
+
+# ------------------------------------------------------------------------------------------------ launches
+def test_launches_are_counted_as_made():
+    def launches(call):
+        before = K.STATS.launches
+        call()
+        return K.STATS.launches - before
+
+    def attend(B, rows, L):
+        att = PagedAttentionForward(PagedAttentionConfig(rows, 64))
+        pool = KvPagePool(L // 16 + 1, KvPageConfig(block_size=16, num_heads=1, head_dim=64), DEV)
+        q = torch.zeros(B, rows, 64, dtype=torch.bfloat16, device=DEV)
+        chain = torch.arange(L // 16 + 1, dtype=torch.int32, device=DEV)
+        lens = torch.full((B,), L + 4, dtype=torch.int32, device=DEV)
+        return lambda: att.forward_shared_prefix(q, pool, chain.expand(B, -1), lens, chain, L)
+
+    assert launches(attend(4, 4, 512)) == 2  # 16 rows: the prefix goes with the tails
+    assert launches(attend(5, 4, 512)) == 3  # 20 rows: tcgen05 takes it
+    assert launches(attend(0, 4, 512)) == 0
+    pools = [KvPagePool(2100, KvPageConfig(block_size=1, num_heads=1, head_dim=8), DEV) for _ in range(129)]
+    assert launches(lambda: copy_pages(pools[:128], [0], [1])) == 1
+    assert launches(lambda: copy_pages(pools, [0], [1])) == 2
+    assert launches(lambda: copy_pages(pools[0], list(range(1025)), list(range(1025, 2050)))) == 2
+    assert launches(lambda: copy_pages(pools, [], [])) == 0
+    for B in (2, 0):
+        p, x = torch.full((B, 2, 8), 0.125, device=DEV), torch.zeros(B, 1, dtype=torch.int64, device=DEV)
+        assert launches(lambda: verify_drafts(p, p[:, :1], x, torch.zeros(B, 2, device=DEV))) == min(B, 1)
+    _ext.check_status(0)
