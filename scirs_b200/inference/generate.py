@@ -148,6 +148,18 @@ class GPTGenerator:
         K.gemm(ln, fp.w("wte"), logits)
         return logits[:, : cfg.vocab_size].float()
 
+    @staticmethod
+    def _draw(logits: torch.Tensor, temperature: float, generator=None) -> list[int]:
+        """A token of each row of logits [n, vocab] at a temperature."""
+        p = torch.softmax(logits / temperature, -1)
+        # A row without a distribution is NaN throughout. On the GPU multinomial would find it by an assertion on
+        # the device, which ends the process's use of it: such a row gets any weights, and no token.
+        bad = torch.isnan(p[:, :1])
+        t = torch.multinomial(p.masked_fill_(bad, 1.0), 1, generator=generator).masked_fill_(bad, -1).view(-1).tolist()
+        if any(x < 0 for x in t):
+            raise InferenceError("the model's probabilities hold no token to draw")
+        return t
+
     def _cache_of(self, seq_ids: list[int]):
         """Tables and lengths of the batch, and the pages that all its chains begin with."""
         dev = self.m.device
@@ -176,10 +188,9 @@ class GPTGenerator:
 
             lg = self._decode(toks, posn, rows, pos, attend)
             if temperature > 0:
-                nxt = torch.multinomial(torch.softmax(lg / temperature, -1), 1, generator=generator).view(-1)
+                out = self._draw(lg, temperature, generator)
             else:
-                nxt = torch.argmax(lg, dim=-1)
-            out = [int(t) for t in nxt.tolist()]
+                out = torch.argmax(lg, dim=-1).tolist()
         for s, t in zip(seq_ids, out):
             self.last_token[s] = t
         return out
@@ -273,9 +284,7 @@ class GPTGenerator:
                 sid, logits = self._prefill(p)
                 ids.append(sid)
                 if temperature > 0:
-                    # (a row each: draws of one row with replacement would check it by an assertion on the device)
-                    probs = torch.softmax(logits / temperature, -1).expand(num_samples, -1)
-                    first = torch.multinomial(probs, 1).view(-1).tolist()
+                    first = self._draw(logits.expand(num_samples, -1), temperature)
                 else:
                     first = [int(torch.argmax(logits))] * num_samples
                 self.last_token[sid] = first[0]

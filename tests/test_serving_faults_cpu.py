@@ -111,11 +111,25 @@ def test_samples_at_a_high_temperature_begin_differently():
     assert gen.pools[0].free_count() == gen.pools[0].total_count()
 
 
-def test_samples_of_logits_that_are_no_numbers_are_refused():
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_samples_of_logits_that_are_no_numbers_are_refused(value):
+    """By the host: an assertion on the device would end all use of it."""
     gen = _generator()
-    gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], torch.full((V,), float("nan"))))(gen._prefill)
-    with pytest.raises(RuntimeError):
+    logits = torch.zeros(V)
+    logits[slice(None) if value < 0 else 5] = value
+    prefill, decode = gen._prefill, gen._decode
+    gen._prefill = lambda p: (prefill(p)[0], logits)
+    with pytest.raises(InferenceError, match="no token"):
         gen.generate([_prompt()], 2, temperature=1.0, num_samples=3)
+    gen._prefill = prefill
+    ids = [gen.add_sequence(_prompt()) for _ in range(2)]
+    gen._decode = lambda *args: torch.stack([decode(*args)[0], logits])
+    with pytest.raises(InferenceError, match="no token"):
+        gen.step(ids, temperature=1.0)
+    n = _prompt().numel()
+    assert [gen.manager.seq_len(s) for s in ids] == [n, n]
+    gen._decode = decode
+    assert len(gen.step(ids, temperature=1.0)) == 2
 
 
 # ------------------------------------------------------------------------------------------------ numbers that are none

@@ -42,14 +42,26 @@ def test_refused_verification_leaves_the_sequences():
 
 
 # ------------------------------------------------------------------------------------------------ samples
-def test_samples_of_logits_that_are_no_numbers_are_refused():
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_samples_of_logits_that_are_no_numbers_are_refused(value):
+    """By the host: an assertion on the device would end all use of it."""
     gen = _generator()
-    nan = torch.full((512,), float("nan"), device=DEV)
-    gen._prefill = (lambda prefill: lambda p: (prefill(p)[0], nan))(gen._prefill)
-    with pytest.raises(RuntimeError):
+    logits = torch.zeros(512, device=DEV)
+    logits[slice(None) if value < 0 else 5] = value
+    prefill, decode = gen._prefill, gen._decode
+    gen._prefill = lambda p: (prefill(p)[0], logits)
+    with pytest.raises(InferenceError, match="no token"):
         gen.generate([_prompt()], 2, temperature=1.0, num_samples=3)
-    torch.cuda.synchronize()  # (the error was the host's: the device goes on)
-    assert float(nan.nan_to_num(1.0).sum()) == 512.0
+    gen._prefill = prefill
+    ids = [gen.add_sequence(_prompt()) for _ in range(2)]
+    gen._decode = lambda *args: torch.stack([decode(*args)[0], logits])
+    with pytest.raises(InferenceError, match="no token"):
+        gen.step(ids, temperature=1.0)
+    n = _prompt().numel()
+    assert [gen.manager.seq_len(s) for s in ids] == [n, n]
+    gen._decode = decode
+    assert len(gen.step(ids, temperature=1.0)) == 2
+    _ext.check_status(0)
 
 
 def test_samples_begin_differently():
