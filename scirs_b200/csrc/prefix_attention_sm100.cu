@@ -125,6 +125,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
   uint64_t* drain = q_empty + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  // a page of the prefix's chain was none of the pool's (at a fixed place: the softmax has no register for its address)
+  __shared__ volatile int lost_flag;
 
   allow_next();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -147,6 +149,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
     mbar_init(q_empty, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
+    lost_flag = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -290,20 +293,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         if (box > 0 && key0 + kBlk <= p.L) {
           const int key = key0 + lane * box;
           const int slot_in_page = key - page_of(p, key) * p.bs;
-          int page = 0;
-          if (lane * box < kBlk) {
-            page = p.pages[page_of(p, key)];
-            if (!input_in_range(page, p.num_pages, p.st, 96)) page = 0;  // (reported)
-          }
+          const bool mine = lane * box < kBlk;
+          const int page = mine ? p.pages[page_of(p, key)] : 0;
+          const bool good = input_in_range(page, p.num_pages, p.st, 96);
           if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
             ok = false;
             break;
           }
           uint64_t* bar = &full[unit % NS];
-          if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+          uint8_t* dst = smem + C::OFF_RING + (unit % NS) * C::TILE + lane * box * 128;
+          const uint32_t lost = __ballot_sync(0xffffffffu, !good);
+          if (lost != 0u) {  // zeros in the box's place; the softmax leaves its keys out
+            if (!good)
+#pragma unroll 1
+              for (int i = 0; i < box * 8; ++i)
+#pragma unroll
+                for (int h = 0; h < HDP / 64; ++h)
+                  *reinterpret_cast<uint4*>(dst + h * (kBlk * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+            lost_flag = 1;
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE - __popc(lost) * box * HDP * 2);
           __syncwarp();
-          if (lane * box < kBlk) {
-            uint8_t* dst = smem + C::OFF_RING + (unit % NS) * C::TILE + lane * box * 128;
+          if (mine && good) {
 #pragma unroll
             for (int h = 0; h < HDP / 64; ++h)
               tma_load_5d(dst + h * (kBlk * 128), (w & 1) ? &map_v : &map_k, bar, 0, slot_in_page, h, I.hk, page);
@@ -316,6 +329,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + i * 32 + lane;
           row[i] = key < p.L ? pool_row(p, p.pages, max_pages, key, I.hk) : -1;
+          if (key < p.L && row[i] < 0) lost_flag = 1;
         }
         if (!mbar_wait(&empty[unit % NS], ((unit / NS) & 1) ^ 1, p.st, 103, abort_flag)) {
           ok = false;
@@ -394,10 +408,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         tc_wait_ld_regs(x + 32);
         tmem_ld_32x32b_x32(s_base + 64, x + 64);
         tmem_ld_32x32b_x32(s_base + 96, x + 96);
-        const int left = p.L - (I.j0 + (STREAMS == 2 ? 2 * j + t : j)) * kBlk;
-        if (left < kBlk) {
+        // keys that are not there: behind the prefix's end, or of a page that is none of the pool's
+        const int key0 = (I.j0 + (STREAMS == 2 ? 2 * j + t : j)) * kBlk;
+        const bool partial = p.L - key0 < kBlk || lost_flag != 0;
+        const auto leave_out = [&](float* v, int first) {
+          const int key = first + lane;
+          const uint32_t there =
+              __ballot_sync(0xffffffffu, key < p.L && (unsigned)p.pages[page_of(p, key)] < (unsigned)p.num_pages);
 #pragma unroll
-          for (int e = 0; e < kBlk / 2; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
+          for (int e = 0; e < 32; ++e) v[e] = (there >> e) & 1u ? v[e] : -INFINITY;
+        };
+        if (partial) {
+          leave_out(sv, key0);
+          leave_out(sv + 32, key0 + 32);
         }
         float m4[4] = {sv[0], sv[1], sv[2], sv[3]};
 #pragma unroll
@@ -409,9 +432,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
         }
         tc_wait_ld_regs(x + 64);
         tc_wait_ld_regs(x + 96);
-        if (left < kBlk) {
-#pragma unroll
-          for (int e = kBlk / 2; e < kBlk; ++e) sv[e] = e < left ? sv[e] : -INFINITY;
+        if (partial) {
+          leave_out(sv + 64, key0 + 64);
+          leave_out(sv + 96, key0 + 96);
         }
 #pragma unroll
         for (int e = kBlk / 2; e < kBlk; e += 8) {

@@ -89,6 +89,8 @@ class PagedAttentionForward:
         its own chain from the first key on. Every head_dim that is a multiple of 8 up to 128, any
         number of query heads per cached head, any page size. bf16; the softmax and the sums are
         kept in fp32. A captured graph keeps prefix_len, and reads the tables and lengths anew.
+        A page id outside of the pool is refused on the CPU; on the GPU its keys are left out, and the
+        next check_status raises.
         """
         c, n = pool.config, self.config
         if q.dim() not in (3, 4) or q.shape[-2] != n.num_heads or q.shape[-1] != n.head_dim:
@@ -145,6 +147,8 @@ def shared_prefix_attention_reference(q, pool: KvPagePool, block_tables, seq_len
         if n - ql + 1 >= prefix_len > 0:
             head = pos < prefix_len
             pages[head] = prefix_pages.long().to(pool.k.device)[pos[head] // bs]
+        if ((pages < 0) | (pages >= pool.k.shape[0])).any():
+            raise InferenceError("a chain names a page outside of the pool")
         k = pool.k[pages, pos % bs].float().repeat_interleave(G, dim=1)
         v = pool.v[pages, pos % bs].float().repeat_interleave(G, dim=1)
         for t in range(ql):

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from scirs_b200.inference import (BlockManager, BlockManagerConfig, GPTGenerator, InferenceError, KvPageConfig,
-                                  KvPagePool, SharedPrefixCache, verify_drafts)
+                                  KvPagePool, PagedAttentionConfig, PagedAttentionForward, SharedPrefixCache,
+                                  verify_drafts)
 from scirs_b200.models.gpt import GPTConfig, GPTModel
 
 V = 128
@@ -237,3 +238,22 @@ def test_verification_refuses_rows_of_more_than_thirty_bits(n, vocab):
 
     with pytest.raises(ValueError, match="2\\^30"):
         verify_drafts(like(1, n + 1, vocab), like(1, n, vocab), like(1, n, dtype=torch.int64), like(1, n + 1))
+
+
+# ------------------------------------------------------------------------------------------------ bad pages
+@pytest.mark.parametrize("bad", [-1, 8, 10 ** 6])
+def test_pages_outside_of_the_pool_are_refused(bad):
+    pool = KvPagePool(8, KvPageConfig(block_size=4, num_heads=2, head_dim=8), "cpu")
+    att = PagedAttentionForward(PagedAttentionConfig(2, 8))
+    tables, lens = torch.tensor([[0, 1, 2, 3]], dtype=torch.int32), torch.tensor([14], dtype=torch.int32)
+    prefix, q = torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, 2, 8)
+    assert att.forward_shared_prefix(q, pool, tables, lens, prefix, 8).shape == q.shape
+    for t, i in ((tables[0], 3), (prefix, 1)):
+        old = int(t[i])
+        t[i] = bad
+        with pytest.raises(InferenceError, match="outside"):
+            att.forward_shared_prefix(q, pool, tables, lens, prefix, 8)
+        t[i] = old
+    tables[0, 3] = bad  # behind the sequence's end
+    lens[0] = 12
+    assert att.forward_shared_prefix(q, pool, tables, lens, prefix, 8).shape == q.shape

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_prefix_serving_gpu import Case
+
 from scirs_b200 import _ext
 from scirs_b200.inference import (GPTGenerator, InferenceError, KvPageConfig, KvPagePool, PagedAttentionConfig,
                                   PagedAttentionForward, copy_pages, verify_drafts)
@@ -130,3 +132,55 @@ def test_launches_are_counted_as_made():
         p, x = torch.full((B, 2, 8), 0.125, device=DEV), torch.zeros(B, 1, dtype=torch.int64, device=DEV)
         assert launches(lambda: verify_drafts(p, p[:, :1], x, torch.zeros(B, 2, device=DEV))) == min(B, 1)
     _ext.check_status(0)
+
+
+# ------------------------------------------------------------------------------------------------ bad pages
+def _exact_without(c, lost):
+    """(output, sum of p |v|) in 64 bits of a Case whose sequences do not see the keys of prefix pages `lost`; the
+    tolerance is the one that Case.check derives."""
+    o = torch.zeros(c.B, c.Q, c.Hkv * c.G, c.HD, dtype=torch.float64)
+    a = torch.zeros_like(o)
+    for b in range(c.B):
+        m = int(c.lens[b])
+        pos = torch.arange(m)
+        page = c.tables[b].long()[pos // c.bs]
+        kept = torch.ones(m, dtype=torch.bool)
+        if m - c.Q + 1 >= c.L:
+            for i in lost:
+                kept &= (pos >= c.L) | (pos // c.bs != i)
+        k, v = c.k[page, pos % c.bs].double(), c.v[page, pos % c.bs].double()
+        for t in range(c.Q):
+            on = kept & (pos < m - c.Q + t + 1)
+            for h in range(c.Hkv * c.G):
+                p = torch.softmax(k[on, h // c.G] @ c.q[b, t, h].double() * c.scale, 0)
+                o[b, t, h], a[b, t, h] = p @ v[on, h // c.G], p @ v[on, h // c.G].abs()
+    return o, a
+
+
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+@pytest.mark.parametrize("B,L,HD,bs,lost", [
+    (3, 90, 64, 16, [2]), (3, 90, 64, 8, [0, 11]), (3, 92, 128, 5, [7]), (3, 90, 40, 16, [5]),  # with the tails
+    (20, 700, 64, 16, [7]), (20, 700, 128, 16, [0, 1, 9, 43]), (20, 700, 128, 128, [3]),  # tcgen05, copies by TMA
+    (70, 640, 64, 64, [9]), (20, 641, 64, 5, [0, 60, 128]), (20, 650, 80, 16, [40])])  # and by cp.async; one block lost
+def test_keys_of_bad_prefix_pages_are_left_out_on_every_path(B, L, HD, bs, lost, bad):
+    c = Case([L + 3 + i % 7 for i in range(B)] + [L - 30], 2, 2, 2, HD, bs, L, seed=L + HD)
+    o, a = _exact_without(c, lost)
+    c.prefix_pages[lost] = bad
+    out = c.run().cpu().double()
+    with pytest.raises(RuntimeError, match="bounds"):
+        _ext.check_status(0)
+    err = (out - o).abs()
+    tol = 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * a + 1e-30
+    assert torch.isfinite(out).all() and (err <= tol).all(), float((err / tol).max())
+
+
+def test_a_block_of_bad_prefix_pages():
+    """No key of the prefix's first two blocks is there, or none of it at all."""
+    for lost in (list(range(16)), list(range(33)), list(range(8, 33))):
+        c = Case([530] * 20, 1, 1, 2, 64, 16, 528, seed=2)
+        o, a = _exact_without(c, lost)
+        c.prefix_pages[lost] = -5
+        out = c.run().cpu().double()
+        with pytest.raises(RuntimeError, match="bounds"):
+            _ext.check_status(0)
+        assert ((out - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * a).all()
