@@ -80,8 +80,8 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)((c >> 3) * Cfg<HDP>::HALF + r * 128 + ((c ^ r) & 7) * 16);
 }
 
-// W: warps of an item; the CTA's four warps take one item together, or one each.
-template <int HDP, int MT, bool TMA, int W>
+// W: warps of an item; the CTA's four warps take one item together, or one each. SPARE: there are spare items.
+template <int HDP, int MT, bool TMA, int W, bool SPARE>
 __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
                                                                              const Params p) {
@@ -100,28 +100,44 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
   // ---- which rows against which keys. Neighbouring items are the cached heads of the same keys, which lie
   // side by side in a page.
   int i = blockIdx.x * (kWarps / W) + warp / W;
-  if (i >= p.items) {
+  if (i >= p.items + (SPARE ? p.spare : 0)) {
     wait_for_previous();
     return;
   }
+  const bool is_spare = SPARE && i >= p.items;
+  if (is_spare) i -= p.items;
   const int hk = i % p.Hkv;
   i /= p.Hkv;
-  const bool is_prefix = i < p.P * p.rt_p;  // (rt_p = 0 when tcgen05 takes the prefix)
-  int r0, r_end, split, b = 0;
+  const bool is_prefix = !is_spare && i < p.P * p.rt_p;  // (rt_p = 0 when tcgen05 takes the prefix)
+  int r0, r_end, split, slot, b = 0;  // (slot: where this part of a row goes)
   const int* pages;
   if (is_prefix) {
-    split = i % p.P;
+    slot = split = i % p.P;
     r0 = i / p.P * M;
     r_end = p.B * p.Q * p.G;
     pages = p.pages;
   } else {
-    i -= p.P * p.rt_p;
-    split = i % p.T;
-    i /= p.T;
-    b = i / p.rt_t;
-    r0 = b * p.Q * p.G + (i - b * p.rt_t) * M;
+    if (is_spare) {  // a part of a row tile of one of the sequences that end inside the prefix
+      const int inside = count_inside(p, lane), parts = inside > 0 ? spare_parts(p, inside) : 0;
+      if (i >= inside * p.rt_t * parts) {
+        wait_for_previous();
+        return;
+      }
+      split = p.T + i % parts;
+      i /= parts;
+      b = nth_inside(p, i / p.rt_t, lane);
+      i %= p.rt_t;
+    } else {
+      i -= p.P * p.rt_p;
+      split = i % p.T;
+      slot = p.P + split;
+      i /= p.T;
+      b = i / p.rt_t;
+      i -= b * p.rt_t;
+    }
+    r0 = b * p.Q * p.G + i * M;
     r_end = (b + 1) * p.Q * p.G;
-    pages = p.tables + (long)b * p.table_stride;
+    pages = p.tables + (long)b * p.max_pages;
   }
   const int max_pages = is_prefix ? p.pages_max : p.max_pages;
 
@@ -139,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     batch = j;
   };
   // the whole tail in one item: its pages can be read before its length is known
-  const bool early = TMA && (is_prefix || p.T == 1);
+  const bool early = TMA && (is_prefix || (p.T == 1 && !is_spare));
   if (early) look_up(0);
 
   int k0, len = 0, ql = 0;
@@ -148,7 +164,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     k1 = min(base + p.per_p, p.L);
   } else {
     const Seq s = seq_from(p, p.lens[b], p.qlens != nullptr ? p.qlens[b] : p.Q, lane == 0 && part_w == 0);
-    const int share = tail_share(p, s);
+    int parts = p.T;
+    if (SPARE && ends_inside(p, s)) {
+      parts += spare_parts(p, count_inside(p, lane));
+      slot = spare_at(p) + split;
+    }
+    const int share = tail_share(s, parts);
     const int first = first_key(s) + split * share;
     k0 = max(first, s.start);
     k1 = min(first + share, s.len);
@@ -457,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
       }
     }
   join();
-  const int slots = p.P + p.T;
+  const int slots = SPARE ? slots_of(p) : p.P + p.T;
   for (int r = part_w; r < M && r0 + r < r_end; r += W) {
     float m = -INFINITY, f[W], l = 0.f;
 #pragma unroll
@@ -469,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
       l += f[w] * mml[(w * M + r) * 2 + 1];
     }
     const int gr = r0 + r, bt = gr / p.G;
-    const long part = ((long)bt * p.H + hk * p.G + gr - bt * p.G) * slots + (is_prefix ? split : p.P + split);
+    const long part = ((long)bt * p.H + hk * p.G + gr - bt * p.G) * slots + slot;
     for (int d = lane * 2; d < p.HD; d += 64) {
       float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
@@ -496,7 +517,7 @@ CUtensorMap pool_map(const Params& p, const bf16* pool, int rows, int halves) {
 }
 
 // W warps to an output row, which take every W-th part.
-template <int W>
+template <int W, bool SPARE>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * (4 / W) + warp / W;
@@ -504,7 +525,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   __shared__ float4 acc_s[4][32];
   __shared__ float den_s[4];
   const int bt = row / p.H, h = row - bt * p.H, b = bt / p.Q, t = bt - b * p.Q;
-  const int slots = p.P + p.T;
+  const int slots = SPARE ? slots_of(p) : p.P + p.T;
   const float* ml = p.part_ml + (long)row * slots * 2;
   const float* po = p.part_o + (long)row * slots * p.HD;
   const Seq s = seq_of(p, b);
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   // a lane reads the maximum of one slot
   const float mine = lane < slots ? ml[2 * lane] : -INFINITY;
   // the slots that hold parts of this row: the prefix's, if the sequence takes part in it, and its tail's
-  int np = 0, nt = 0;
+  int np = 0, nt = 0, tail_at = p.P;
   if (t < s.ql) {
     if (s.start == p.L) {
       np = p.P;
@@ -523,16 +544,21 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
         np = ((first + p.tc_blocks - 1) / p.tc_share - first / p.tc_share + 1) * p.tc_streams;
       }
     }
-    const int n = tail_keys(s), share = tail_share(p, s);
+    int parts = p.T;
+    if (SPARE && ends_inside(p, s)) {
+      parts += spare_parts(p, count_inside(p, lane));
+      tail_at = spare_at(p);
+    }
+    const int n = tail_keys(s), share = tail_share(s, parts);
     if (n > 0) nt = (n + share - 1) / share;
   }
-  const auto used = [&](int i) { return i < np || (i >= p.P && i < p.P + nt); };
+  const auto used = [&](int i) { return i < np || (i >= tail_at && i < tail_at + nt); };
   float m = used(lane) ? mine : -INFINITY;
   for (int i = lane + 32; i < slots; i += 32)
     if (used(i)) m = fmaxf(m, ml[2 * i]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
-  const auto slot_of = [&](int j) { return j < np ? j : p.P + j - np; };
+  const auto slot_of = [&](int j) { return j < np ? j : tail_at + j - np; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.f;
   const bool on = 4 * lane < p.HD;
@@ -587,6 +613,12 @@ constexpr int64_t kTcRows = 16, kTcKeys = 512, kTcLong = 32768;
 // Keys of an item, at least (16 rows, 1024 keys of the prefix: 256 instead of 128 takes 12.8 us, not 10.8), and
 // parts of a row's prefix, at most, where they fill the device (8192 keys in 32 parts instead of 64: 22 -> 15 us).
 constexpr int64_t kMinKeys = 128, kParts = 32;
+// Keys that a warp of a sequence that ends inside the prefix walks, at most, before spare items take parts of them (2048
+// take 0.15 ms). With one such sequence of 99990 tokens of 16 a call takes 181 us, without spare items 1484; 3 of 256
+// inside 32768 tokens 311 us, not 705; in tails of a warp 155, not 1616. Where no sequence ends inside, the kernels with
+// spare items cost 0.3 to 1 % behind long prefixes, but 4 to 7 % where items are short or have 32 rows (1024 sequences
+// behind 2048 tokens 94 -> 101 us, 64 x 5 x 8 heads behind 4096 118 -> 123): those go without.
+constexpr int64_t kWalk = 2048;
 // Up to here a warp joins a row's parts, above four do (2048 rows of 20 parts: 9 us with four).
 constexpr int kFewParts = 8;
 
@@ -647,7 +679,7 @@ std::tuple<torch::Tensor, int64_t> paged_prefix_attention(torch::Tensor q, torch
   p.q_sb = q.stride(0);
   p.q_st = q.stride(1);
   p.q_sh = q.stride(2);
-  p.table_stride = p.max_pages = (int)max_pages;
+  p.max_pages = (int)max_pages;
   p.num_pages = (int)num_pages;
   p.B = (int)B;
   p.Q = (int)Q;
@@ -684,15 +716,19 @@ std::tuple<torch::Tensor, int64_t> paged_prefix_attention(torch::Tensor q, torch
   const int run = p.bs & -p.bs;
   p.box = (HD == 64 || HD == 128) && run >= 8 ? std::min(run, prefix::kTile) : 0;
   if (tc) prefix::plan_prefix_tc(p, sms);
-  const int slots = p.P + p.T;
-  auto parts = at::empty({B * Q * H * slots * (HD + 2)}, q.options().dtype(at::kFloat));
-  p.part_o = parts.data_ptr<float>();
-  p.part_ml = p.part_o + B * Q * H * slots * HD;
   const int64_t items = Hkv * ((int64_t)p.rt_p * p.P + B * p.rt_t * p.T);
   TORCH_CHECK(items < (1LL << 30), "paged attention: too large");
   p.items = (int)items;
   // many short tails (no longer than an item's smallest share, more than two rounds of CTAs): a warp each
   const bool solo = mt == 1 && p.rt_p == 0 && span <= kMinKeys && items > ctas;
+  // a spare item for each SM where the T parts of a sequence that ends inside the prefix could have more than kWalk
+  // keys a warp
+  if (L > kWalk * p.T * (solo ? 1 : prefix::kWarps))
+    p.spare = (int)(sms * (solo ? prefix::kWarps : 1) / Hkv * Hkv);
+  const int slots = prefix::slots_of(p);
+  auto parts = at::empty({B * Q * H * slots * (HD + 2)}, q.options().dtype(at::kFloat));
+  p.part_o = parts.data_ptr<float>();
+  p.part_ml = p.part_o + B * Q * H * slots * HD;
   if (tc) {
     prefix::launch_prefix_tc(p, cur_stream());
   }
@@ -702,38 +738,46 @@ std::tuple<torch::Tensor, int64_t> paged_prefix_attention(torch::Tensor q, torch
     map_k = prefix::pool_map(p, p.k, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
     map_v = prefix::pool_map(p, p.v, p.box, p.box == prefix::kTile ? (int)HD / 64 : 1);
   }
-#define SCIRS_ITEMS(HDP_, MT_, TMA_, W_)                                                                             \
+#define SCIRS_ITEMS(HDP_, MT_, TMA_, W_, SPARE_)                                                                     \
   {                                                                                                                  \
-    auto kern = prefix::item_kernel<HDP_, MT_, TMA_, W_>;                                                            \
+    auto kern = prefix::item_kernel<HDP_, MT_, TMA_, W_, SPARE_>;                                                    \
     constexpr int smem = prefix::Cfg<HDP_>::smem(MT_), each = prefix::kWarps / W_;                                   \
     set_max_smem((const void*)kern, smem);                                                                           \
-    prefix::launch(kern, (unsigned)((items + each - 1) / each), prefix::kThreads, smem, st, tc, map_k, map_v, p);    \
+    prefix::launch(kern, (unsigned)((items + p.spare + each - 1) / each), prefix::kThreads, smem, st, tc, map_k,     \
+                   map_v, p);                                                                                        \
   }
-#define SCIRS_ITEMS_MT(HDP_, TMA_)                  \
+#define SCIRS_ITEMS_MT(HDP_, TMA_, SPARE_)          \
   if (solo)                                         \
-    SCIRS_ITEMS(HDP_, 1, TMA_, 1)                   \
+    SCIRS_ITEMS(HDP_, 1, TMA_, 1, SPARE_)           \
   else if (mt == 1)                                 \
-    SCIRS_ITEMS(HDP_, 1, TMA_, 4)                   \
+    SCIRS_ITEMS(HDP_, 1, TMA_, 4, SPARE_)           \
   else                                              \
-    SCIRS_ITEMS(HDP_, 2, TMA_, 4)
-  if (p.box > 0) {
-    if (HD == 64) {
-      SCIRS_ITEMS_MT(64, true)
-    } else {
-      SCIRS_ITEMS_MT(128, true)
-    }
-  } else if (HD <= 64) {
-    SCIRS_ITEMS_MT(64, false)
+    SCIRS_ITEMS(HDP_, 2, TMA_, 4, SPARE_)
+// four warps to a row where its parts are many, one where they are few
+#define SCIRS_ATTEND(SPARE_)                                                                                   \
+  if (p.box > 0) {                                                                                             \
+    if (HD == 64) {                                                                                            \
+      SCIRS_ITEMS_MT(64, true, SPARE_)                                                                         \
+    } else {                                                                                                   \
+      SCIRS_ITEMS_MT(128, true, SPARE_)                                                                        \
+    }                                                                                                          \
+  } else if (HD <= 64) {                                                                                       \
+    SCIRS_ITEMS_MT(64, false, SPARE_)                                                                          \
+  } else {                                                                                                     \
+    SCIRS_ITEMS_MT(128, false, SPARE_)                                                                         \
+  }                                                                                                            \
+  if (p.P + p.T > kFewParts)                                                                                   \
+    prefix::launch(prefix::combine_kernel<4, SPARE_>, (unsigned)(B * Q * H), 128, 0, st, true, p);             \
+  else                                                                                                         \
+    prefix::launch(prefix::combine_kernel<1, SPARE_>, (unsigned)((B * Q * H + 3) / 4), 128, 0, st, true, p);
+  if (p.spare > 0) {
+    SCIRS_ATTEND(true)
   } else {
-    SCIRS_ITEMS_MT(128, false)
+    SCIRS_ATTEND(false)
   }
+#undef SCIRS_ATTEND
 #undef SCIRS_ITEMS_MT
 #undef SCIRS_ITEMS
-  // four warps to a row where its parts are many, one where they are few
-  if (slots > kFewParts)
-    prefix::launch(prefix::combine_kernel<4>, (unsigned)(B * Q * H), 128, 0, st, true, p);
-  else
-    prefix::launch(prefix::combine_kernel<1>, (unsigned)((B * Q * H + 3) / 4), 128, 0, st, true, p);
   return {out, tc ? 3 : 2};
 }
 

@@ -10,6 +10,7 @@ namespace prefix {
 using bf16 = __nv_bfloat16;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kTile = 16;  // keys per step of a warp: split lengths are multiples
+constexpr int kSpareParts = 32;  // parts of a row that spare items take, at most, where items take the prefix too
 constexpr float kRaise = 8.f;  // a running maximum is raised only past 2^8
 
 struct Params {
@@ -18,7 +19,7 @@ struct Params {
   const int *tables, *lens, *qlens, *pages;  // qlens may be null: Q each
   float *part_o, *part_ml;                   // [B Q H, slots, HD], [B Q H, slots, 2]
   long q_sb, q_st, q_sh;                     // element strides of q
-  int table_stride, max_pages, num_pages;
+  int max_pages, num_pages;                  // (tables are [B, max_pages])
   int B, Q, H, Hkv, G, HD, bs;
   int L;                // tokens of the prefix
   int P, T;             // splits of the prefix and of a tail, and their slots: 0 .. P - 1, P .. P + T - 1
@@ -26,6 +27,7 @@ struct Params {
   int rt_p, rt_t;       // item_kernel: row tiles of the prefix (0: tcgen05 takes it), of a tail
   int pages_max;        // pages of the prefix
   int items;            // of item_kernel
+  int spare;            // items behind those, which take more parts of the sequences that end inside the prefix
   int box;              // keys of a TMA box (0: cp.async)
   uint32_t bs_mul;      // division by bs (see page_of)
   int bs_shift;
@@ -61,8 +63,42 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
 // keys from there, and a split's share of them.
 __device__ __forceinline__ int first_key(const Seq& s) { return s.start & ~(kTile - 1); }
 __device__ __forceinline__ int tail_keys(const Seq& s) { return s.len > s.start ? s.len - first_key(s) : 0; }
-__device__ __forceinline__ int tail_share(const Params& p, const Seq& s) {
-  return ((tail_keys(s) + p.T - 1) / p.T + kTile - 1) / kTile * kTile;
+__device__ __forceinline__ int tail_share(const Seq& s, int parts) {
+  return ((tail_keys(s) + parts - 1) / parts + kTile - 1) / kTile * kTile;
+}
+
+// A sequence that ends inside the prefix is read by itself from its first key, up to L of them, where T goes by the
+// tails behind the prefix. Only the device knows which these are: where they would take long, their keys are cut into
+// T + spare_parts shares, and the spare items, as many to each of them as there are for all that the batch has, take
+// those behind the T-th.
+__device__ __forceinline__ bool ends_inside(const Params& p, const Seq& s) { return s.start != p.L && s.len > 0; }
+
+// How many there are (the same in all lanes).
+__device__ __forceinline__ int count_inside(const Params& p, int lane) {
+  int n = 0;
+#pragma unroll 1
+  for (int b = lane; b < p.B; b += 32) n += ends_inside(p, seq_of(p, b));
+  return __reduce_add_sync(0xffffffffu, n);
+}
+// The k-th of them, from 0.
+__device__ __forceinline__ int nth_inside(const Params& p, int k, int lane) {
+  for (int b0 = 0;; b0 += 32) {
+    const int b = b0 + lane;
+    const uint32_t on = __ballot_sync(0xffffffffu, b < p.B && ends_inside(p, seq_of(p, b)));
+    if (k < __popc(on)) return b0 + __fns(on, 0, k + 1);
+    if (b0 + 32 >= p.B) return 0;  // (not reached)
+    k -= __popc(on);
+  }
+}
+__device__ __forceinline__ int spare_parts(const Params& p, int inside) {
+  return min(p.spare / (inside * p.Hkv * p.rt_t), p.rt_p == 0 ? p.P : kSpareParts);
+}
+// Where the slots of such a row begin: with tcgen05 (rt_p = 0) at the prefix's, of which it has none; items write
+// their part of every row.
+__device__ __forceinline__ int spare_at(const Params& p) { return p.rt_p == 0 ? 0 : p.P + p.T; }
+// Slots of a row.
+__host__ __device__ __forceinline__ int slots_of(const Params& p) {
+  return p.P + p.T + (p.spare > 0 && p.rt_p > 0 ? p.T + kSpareParts : 0);
 }
 
 // key / bs for 0 <= key < 2^31: multiplication by the rounded-up reciprocal (Granlund & Montgomery, 1994).

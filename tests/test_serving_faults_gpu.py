@@ -184,3 +184,87 @@ def test_a_block_of_bad_prefix_pages():
         with pytest.raises(RuntimeError, match="bounds"):
             _ext.check_status(0)
         assert ((out - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * a).all()
+
+
+# ------------------------------------------------------------------------------------------------ shorter than the prefix
+@pytest.mark.parametrize("lens,Q,Hkv,G,HD,bs,L,qlens", [
+    # tcgen05 takes the prefix; one, some, most and all of the sequences end inside it
+    pytest.param([2100] * 19 + [2040], 1, 2, 2, 128, 16, 2048, None, id="one_of_twenty"),
+    pytest.param([2100, 3, 2060, 1999, 0, 1500] * 5, 2, 2, 2, 64, 16, 2048, [2, 2, 1, 2, 0, 1] * 5, id="a_third"),
+    pytest.param([2047 - i for i in range(29)] + [2050], 1, 1, 8, 128, 16, 2048, None, id="all_but_one"),
+    pytest.param([1600 + i for i in range(40)], 4, 1, 2, 64, 24, 1640, [4, 1, 2, 3] * 10, id="all"),
+    pytest.param([2010, 2051, 2049, 1], 5, 2, 8, 128, 16, 2048, [5, 5, 1, 1], id="three_row_tiles_of_a_tail"),
+    pytest.param([1800, 1700, 30] * 4, 2, 1, 2, 80, 16, 1750, None, id="head_dim_80"),
+    pytest.param([1800, 1700, 30] * 4, 2, 2, 2, 64, 5, 1750, None, id="pages_of_five"),
+    # the prefix goes with the tails (up to 16 rows)
+    pytest.param([3000, 2980, 2, 2999], 1, 2, 4, 64, 16, 2990, None, id="items"),
+    pytest.param([3000, 2980, 2, 2999], 2, 1, 2, 128, 5, 2990, [2, 2, 1, 2], id="items_cp_async"),
+    # a warp a tail
+    pytest.param([1300 if i % 9 else 1100 + i for i in range(100)], 1, 16, 1, 64, 16, 1250, None, id="warps"),
+    pytest.param([1300 if i % 50 else 900 for i in range(100)], 2, 16, 1, 128, 16, 1250, [1 + i % 2 for i in range(100)], id="warps_two_queries"),
+    pytest.param([20000, 20040, 19000], 1, 8, 8, 128, 16, 20010, None, id="long"),
+    # more keys than one item takes
+    pytest.param([9100] * 11 + [9000], 1, 1, 2, 128, 16, 9040, None, id="long_one_of_twelve"),
+    pytest.param([9100, 8300, 3, 9050, 0, 8999] * 2, 2, 1, 2, 64, 16, 9040, [2, 2, 1, 2, 0, 1] * 2, id="long_half"),
+    pytest.param([9000 - 40 * i for i in range(12)], 1, 1, 2, 64, 16, 9040, None, id="long_all"),
+    pytest.param([8400, 9050, 8999, 1], 5, 1, 8, 128, 16, 9040, [5, 5, 1, 1], id="long_three_row_tiles"),
+    pytest.param([9100, 9000, 8500, 17], 2, 1, 3, 80, 16, 9040, None, id="long_head_dim_80"),
+    pytest.param([9100, 9000, 8500, 17], 2, 1, 3, 64, 5, 9040, None, id="long_pages_of_five"),
+    pytest.param([9100, 9000, 8500], 1, 2, 4, 64, 16, 9040, None, id="long_items"),
+    pytest.param([9100, 9000, 8500], 2, 1, 2, 128, 5, 9040, [2, 2, 1], id="long_items_cp_async"),
+    pytest.param([2300 if i % 9 else 2100 + i for i in range(100)], 1, 16, 1, 64, 16, 2250, None, id="long_warps"),
+    pytest.param([2300 if i % 50 else 2200 for i in range(100)], 2, 16, 1, 128, 16, 2250, [1 + i % 2 for i in range(100)], id="long_warps_two_queries"),
+])
+def test_sequences_that_end_inside_a_long_prefix(lens, Q, Hkv, G, HD, bs, L, qlens):
+    c = Case(lens, Q, Hkv, G, HD, bs, L, qlens, seed=L + Q)
+    first = c.run()
+    c.check(first)
+    pool = c.pool()
+    assert all(torch.equal(c.run(pool=pool), first) for _ in range(3))
+
+
+def test_a_sequence_that_ends_inside_the_prefix_in_a_graph():
+    """A graph captured with lengths behind the prefix is replayed with some inside it, and the other way round."""
+    c = Case([9100, 9060, 9070, 9060] * 5, 1, 1, 2, 64, 16, 9040, seed=6)
+    pool = c.pool()
+    c.k[:], c.v[:] = torch.nan_to_num(c.k), torch.nan_to_num(c.v)
+    args = [t.to(DEV) for t in (c.q, c.tables, c.lens, c.prefix_pages)]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = c.att.forward_shared_prefix(args[0], pool, args[1], args[2], args[3], c.L)
+    for lens in ([9100, 9030, 9070, 5] * 5, [9000] * 20, [9100, 9060, 9070, 9060] * 5):
+        c.lens = torch.tensor(lens, dtype=torch.int32)
+        args[2].copy_(c.lens)
+        gr.replay()
+        torch.cuda.synchronize()
+        c.check(out)
+
+
+def test_a_sequence_that_ends_inside_the_prefix_does_not_hold_up_the_batch():
+    """Read by one item it took 14 times what the others take; the parts that the device's items share, less than twice."""
+    B, Hkv, G, HD, bs, L = 16, 8, 5, 128, 16, 65536
+    n = L // bs
+    pool = KvPagePool(2 * n + B, KvPageConfig(block_size=bs, num_heads=Hkv, head_dim=HD), DEV)
+    pool.k.normal_()
+    pool.v.normal_()
+    front = torch.arange(n, dtype=torch.int32, device=DEV)
+    tables = torch.cat([front.expand(B, -1), 2 * n + torch.arange(B, dtype=torch.int32, device=DEV)[:, None]], 1)
+    tables[-1, :n] += n
+    att = PagedAttentionForward(PagedAttentionConfig(Hkv * G, HD))
+    q = torch.randn(B, Hkv * G, HD, device=DEV).to(torch.bfloat16)
+
+    def time(last):
+        lens = torch.tensor([L + 7] * (B - 1) + [last], dtype=torch.int32, device=DEV)
+        took = []
+        for i in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            att.forward_shared_prefix(q, pool, tables, lens, front, L)
+            b.record()
+            torch.cuda.synchronize()
+            took.append(a.elapsed_time(b))
+        return sorted(took)[3]
+
+    behind, inside = time(L + 7), time(L - 9)
+    _ext.check_status(0)
+    assert inside < 5 * behind, (inside, behind)
