@@ -123,10 +123,15 @@ class PagedAttentionForward:
 
     def forward_manager_shared(self, q: torch.Tensor, manager: BlockManager, seq_ids: list[int],
                                q_lens: torch.Tensor | None = None):
-        """forward_shared_prefix for sequences of a BlockManager, over the pages that they share."""
+        """forward_shared_prefix for sequences of a BlockManager, over the pages that they share. The
+        prefix ends where the first of the queries stands: pages may be shared up to the newest token
+        (forks that have not been written to, a single sequence), and a sequence with a query inside the
+        prefix would be read by itself."""
         manager.sync()
         dev = manager.block_tables.device
         pages, n = manager.shared_prefix(seq_ids)
+        queries = q.shape[1] if q.dim() == 4 else 1
+        n = max(0, min([n] + [manager.seq_len(s) - queries + 1 for s in seq_ids]))
         rows = torch.tensor([manager.row_of(s) for s in seq_ids], dtype=torch.long, device=dev)
         return self.forward_shared_prefix(q, manager.pool, manager.block_tables[rows], manager.seq_lens[rows],
                                           torch.tensor(pages, dtype=torch.int32, device=dev), n, q_lens)

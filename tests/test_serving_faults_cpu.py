@@ -257,3 +257,32 @@ def test_pages_outside_of_the_pool_are_refused(bad):
     tables[0, 3] = bad  # behind the sequence's end
     lens[0] = 12
     assert att.forward_shared_prefix(q, pool, tables, lens, prefix, 8).shape == q.shape
+
+
+# ------------------------------------------------------------------------------------------------ the shared prefix
+@pytest.mark.parametrize("queries", [1, 3, 20])
+def test_the_managers_prefix_ends_in_front_of_the_queries(queries, monkeypatch):
+    """Forks without tokens of their own, and one sequence alone, share full pages up to the newest token."""
+    pool = KvPagePool(16, KvPageConfig(block_size=4, num_heads=2, head_dim=8), "cpu")
+    bm = BlockManager(pool, BlockManagerConfig(4, 8))
+    bm.allocate_sequence(0)
+    kv = torch.randn(16, 2, 8, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    bm.append([0], [16], kv, kv.flip(0))
+    bm.fork_sequence(0, 1)
+    att = PagedAttentionForward(PagedAttentionConfig(4, 8))
+    seen = []
+    shared = PagedAttentionForward.forward_shared_prefix
+
+    def spy(self, q, pool, tables, lens, pages, prefix_len, *rest):
+        seen.append(prefix_len)
+        return shared(self, q, pool, tables, lens, pages, prefix_len, *rest)
+
+    monkeypatch.setattr(PagedAttentionForward, "forward_shared_prefix", spy)
+    for seqs in ([0, 1], [0]):
+        q = torch.randn(len(seqs), queries, 4, 8, generator=torch.Generator().manual_seed(1))
+        out = att.forward_manager_shared(q, bm, seqs)
+        assert seen.pop() == max(0, 16 - queries + 1)  # every query stands behind it
+        none = torch.zeros(0, dtype=torch.int32)
+        want = shared(att, q, pool, bm.block_tables[: len(seqs)][[bm.row_of(s) for s in seqs]],
+                      bm.seq_lens[[bm.row_of(s) for s in seqs]], none, 0)
+        assert torch.equal(out, want)
