@@ -450,6 +450,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HDP>::ctas(MT)) item_kernel(cons
     }
   }
 
+  // (a wait gave up: the copies that are still on their way land before the rings are written or left)
+  for (; TMA && flying > 0; --flying) {
+    mbar_wait(&full[s], phase, p.st, 97, nullptr);
+    if (++s == C::STAGES) {
+      s = 0;
+      phase ^= 1;
+    }
+  }
+
   // ---- join the item's warps (their rings are free now), write this split's part of every row
   float* mo = reinterpret_cast<float*>(W == 1 ? ring : smem);  // [part][M][HDP]
   float* mml = mo + W * M * HDP;                               // [part][M][2]

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
     const bf16* src = (w & 1) ? p.v : p.k;
     const uint32_t ring = smem_u32(smem + C::OFF_RING);
     const int max_pages = (p.L + p.bs - 1) / p.bs;
-    int blk = 0;
+    int blk = 0, last = -1;  // (unit of the last copies by TMA)
     bool ok = true;
     for (int u = u_begin; u < u_end && ok;) {
       const TcItem I = tc_item<STREAMS>(p, u, u_end);
@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
             for (int h = 0; h < HDP / 64; ++h)
               tma_load_5d(dst + h * (kBlk * 128), (w & 1) ? &map_v : &map_k, bar, 0, slot_in_page, h, I.hk, page);
           }
+          last = unit;
           continue;
         }
         // this lane looks four keys' rows up
@@ -354,6 +355,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) prefix_tc_kernel(const __grid_c
       blk += I.n;
       u += I.n;
     }
+    // (a wait gave up: the copies that are still on their way land before the ring is left)
+    if (!ok)
+      for (int unit = last; unit >= 0 && unit > last - NS; unit -= 4)
+        mbar_wait(&full[unit % NS], (unit / NS) & 1, p.st, 107, nullptr);
   } else {
     setmaxnreg_inc<kRegsSoftmax>();
     // ---------------------------------------------------------------- softmax
