@@ -847,7 +847,7 @@ static void launch_epi(int epi, const Maps& m, const Args& args, int grid, cudaS
       if (!A_MN && !B_MN) launch_t<BN, 0, 0, EPI_ROPE>(m, args, grid, s);
       else TORCH_CHECK(false, "the RoPE epilogue takes K-major operands");
       break;
-    default: TORCH_CHECK(false, "bad epilogue ", epi);
+    default: TORCH_CHECK(false, "bad epilogue ", num(epi));
   }
 }
 
@@ -908,7 +908,7 @@ static void launch_pair_epi(int epi, const Maps& m, const Args& args, int grid, 
       if (!A_MN && !B_MN) launch_pair_t<0, 0, EPI_ROPE>(m, args, grid, s);
       else TORCH_CHECK(false, "the RoPE epilogue takes K-major operands");
       break;
-    default: TORCH_CHECK(false, "bad epilogue ", epi);
+    default: TORCH_CHECK(false, "bad epilogue ", num(epi));
   }
 }
 
@@ -963,7 +963,7 @@ static void launch_tp(int a_mn, int b_mn, int epi, const Maps& m, const PeerMaps
   else if (!a_mn && b_mn && epi == EPI_BF16) launch_tp_t<0, 1, EPI_BF16>(m, pm, args, grid, s);
   else if (!a_mn && b_mn && epi == EPI_DGELU) launch_tp_t<0, 1, EPI_DGELU>(m, pm, args, grid, s);
   else if (a_mn && b_mn && epi == EPI_F32) launch_tp_t<1, 1, EPI_F32>(m, pm, args, grid, s);
-  else TORCH_CHECK(false, "tensor-parallel GEMM form not supported: a_mn=", a_mn, " b_mn=", b_mn, " epi=", epi);
+  else TORCH_CHECK(false, "tensor-parallel GEMM form not supported: a_mn=", num(a_mn), " b_mn=", num(b_mn), " epi=", num(epi));
 }
 
 // EPI_ROPE arguments: fp32 [S, hd/2] cos / sin tables, hd a multiple of 64
@@ -1086,7 +1086,7 @@ void gemm_tp(torch::Tensor a, torch::Tensor b, torch::Tensor out, int64_t a_mn, 
   const int64_t K = (ap && a_mn) ? Kl * world : Kl;
   const int64_t Kb = b_mn ? b.size(0) * (bp ? world : 1) : b.size(1);
   const int64_t N = b_mn ? b.size(1) : b.size(0);
-  TORCH_CHECK(K == Kb, "gemm K mismatch: ", K, " vs ", Kb);
+  TORCH_CHECK(K == Kb, "gemm K mismatch: ", num(K), " vs ", num(Kb));
   TORCH_CHECK(N % 8 == 0 && K % 8 == 0, "tensor-parallel gemm needs K and N multiples of 8");
   TORCH_CHECK(!((ap && !a_mn) || rs) || M % (BM * world) == 0, "row-split operands need M % (128*world) == 0");
   if (ap) TORCH_CHECK(a_mn ? (a.size(0) % BK == 0) : (a.size(0) % BM == 0), "segment not tile aligned");
@@ -1263,7 +1263,7 @@ static void gemm_tc_impl(torch::Tensor a, torch::Tensor b, torch::Tensor out, in
   const int64_t K = a_mn ? a.size(0) : a.size(1);
   const int64_t N = b_mn ? b.size(1) : b.size(0);
   const int64_t Kb = b_mn ? b.size(0) : b.size(1);
-  TORCH_CHECK(K == Kb, "gemm K mismatch: ", K, " vs ", Kb);
+  TORCH_CHECK(K == Kb, "gemm K mismatch: ", num(K), " vs ", num(Kb));
   TORCH_CHECK(out.size(0) == M && out.size(1) == N, "gemm out shape mismatch");
   // TMA: the contiguous dimension of every operand must span a multiple of
   // 16 bytes (N is the output's contiguous dimension)

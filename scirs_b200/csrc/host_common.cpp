@@ -62,7 +62,7 @@ CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t i
                          uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                          CUtensorMapSwizzle swizzle) {
   TORCH_CHECK((reinterpret_cast<uintptr_t>(base) & 15) == 0, "TMA base address must be 16-byte aligned");
-  TORCH_CHECK(row_stride_bytes % 16 == 0, "TMA row stride must be a multiple of 16 bytes, got ", row_stride_bytes);
+  TORCH_CHECK(row_stride_bytes % 16 == 0, "TMA row stride must be a multiple of 16 bytes, got ", num(row_stride_bytes));
   CUtensorMap m;
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_stride_bytes};
@@ -71,8 +71,8 @@ CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t i
   CUresult r = get_encode_fn()(&m, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", (int)r, " (inner=", inner,
-              " outer=", outer, " stride=", row_stride_bytes, " box=", box_inner, "x", box_outer, ")");
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", num((int)r), " (inner=", num(inner),
+              " outer=", num(outer), " stride=", num(row_stride_bytes), " box=", num(box_inner), "x", num(box_outer), ")");
   return m;
 }
 

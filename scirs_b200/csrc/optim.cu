@@ -219,7 +219,7 @@ void optim_step(int64_t mode, torch::Tensor params, torch::Tensor state1, torch:
     SCIRS_OPT_CASE(OPT_SGD)
     SCIRS_OPT_CASE(OPT_RMSPROP)
     SCIRS_OPT_CASE(OPT_ADAGRAD)
-    default: TORCH_CHECK(false, "unknown optimizer mode ", mode);
+    default: TORCH_CHECK(false, "unknown optimizer mode ", num(mode));
   }
 #undef SCIRS_OPT_CASE
 }

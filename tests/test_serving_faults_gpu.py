@@ -268,3 +268,14 @@ def test_a_sequence_that_ends_inside_the_prefix_does_not_hold_up_the_batch():
     behind, inside = time(L + 7), time(L - 9)
     _ext.check_status(0)
     assert inside < 5 * behind, (inside, behind)
+
+
+# ------------------------------------------------------------------------------------------------ messages
+def test_refusals_that_print_numbers():
+    """Operands that do not match are an error with their sizes in it."""
+    a, b = (torch.zeros(128, k, dtype=torch.bfloat16, device=DEV) for k in (64, 72))
+    out = torch.zeros(128, 128, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="64 vs 72"):
+        K.gemm(a, b, out)
+    with pytest.raises(RuntimeError, match="epilogue 99"):
+        K.gemm(a, a, out, epi=99)
