@@ -8,7 +8,8 @@ attention over the sequence's page chain -> projection GEMM (+residual) ->
 LayerNorm -> GELU MLP GEMMs -> final LayerNorm -> LM head -> next token.
 All layers share one page table (the pages of layer l live in layer l's
 pool at the same page ids). Sequences can be forked (several samples of one
-prompt share its pages, and a step reads them once), and `verify` feeds a few
+prompt share its pages; a step of samples of one prompt reads them once, a
+step over several prompts reads each chain by itself), and `verify` feeds a few
 drafted tokens per sequence at once and keeps those that the model confirms.
 
 Reference parity: the reference generates with its (placeholder) GPT on the
@@ -106,7 +107,8 @@ class GPTGenerator:
 
     def fork(self, seq_id: int) -> int:
         """A copy of a sequence (its tokens and its pending one) that goes its own way from here. The
-        two share their pages until one of them writes into one; step reads what a batch shares once."""
+        two share their pages until one of them writes into one; a step whose sequences all begin with
+        the same pages reads those once."""
         sid = self._next_id
         self.manager.fork_sequence(seq_id, sid)
         self._next_id += 1
@@ -165,8 +167,8 @@ class GPTGenerator:
         dev = self.m.device
         idx = torch.tensor([self.manager.row_of(s) for s in seq_ids], dtype=torch.long, device=dev)
         pages, shared = self.manager.shared_prefix(seq_ids) if len(seq_ids) > 1 else ([], 0)
-        return (self.manager.block_tables[idx].contiguous(), self.manager.seq_lens[idx].contiguous(),
-                torch.tensor(pages, dtype=torch.int32, device=dev), shared)
+        pages = torch.tensor(pages, dtype=torch.int32).to(dev) if shared else idx.new_empty(0, dtype=torch.int32)
+        return (self.manager.block_tables[idx].contiguous(), self.manager.seq_lens[idx].contiguous(), pages, shared)
 
     @torch.no_grad()
     def step(self, seq_ids: list[int], temperature: float = 0.0, generator=None) -> list[int]:
@@ -182,7 +184,9 @@ class GPTGenerator:
             bt, sl, pages, shared = self._cache_of(seq_ids)
 
             def attend(q, pool):
-                if shared:  # forked sequences: the pages they all begin with are read once
+                # Forked sequences: the pages they all begin with are read once. One shared page is enough: 2 to 64
+                # sequences of 40 to 1000 tokens, 12 heads of 64, 16 to 976 shared: 11 to 73 us, by themselves 20 to 214.
+                if shared:
                     return self.attn.forward_shared_prefix(q, pool, bt, sl, pages, shared)
                 return self.attn.forward_batch(q.contiguous(), pool, bt, sl)
 

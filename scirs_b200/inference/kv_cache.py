@@ -253,6 +253,8 @@ class BlockManager:
         """The leading pages that the chains of all these sequences have in common and are full in
         every one of them, and how many tokens they hold."""
         bs = self.pool.config.block_size
+        if any(self._pages[s][0] != self._pages[seq_ids[0]][0] for s in seq_ids):  # (the usual case first)
+            return [], 0
         common = min(self._lens[s] for s in seq_ids) // bs if seq_ids else 0
         first = self._pages[seq_ids[0]][:common] if common else []
         for s in seq_ids[1:]:
@@ -351,6 +353,8 @@ class BlockManager:
         """(sequence, index in its chain) of the shared pages that sequences growing to `lens` tokens
         write; the last holder of a page keeps it."""
         bs, out = self.pool.config.block_size, []
+        if not self.pool._shared:
+            return out
         refs: dict[int, int] = {}
         for s, end in lens.items():
             pages = self._pages[s]

@@ -286,3 +286,31 @@ def test_the_managers_prefix_ends_in_front_of_the_queries(queries, monkeypatch):
         want = shared(att, q, pool, bm.block_tables[: len(seqs)][[bm.row_of(s) for s in seqs]],
                       bm.seq_lens[[bm.row_of(s) for s in seqs]], none, 0)
         assert torch.equal(out, want)
+
+
+def test_sequences_that_share_nothing_are_not_walked(monkeypatch):
+    """Growing them asks for no page's references, and nothing of their chains but the first pages is compared."""
+    pool = KvPagePool(64, KvPageConfig(block_size=4, num_heads=1, head_dim=8), "cpu")
+    bm = BlockManager(pool, BlockManagerConfig(4, 16))
+
+    class Chain(list):
+        def __getitem__(self, i):
+            assert i == 0
+            return list.__getitem__(self, i)
+
+    for s in range(3):
+        bm.allocate_sequence(s)
+        bm.reserve([s], [14])
+        bm._pages[s] = Chain(bm._pages[s])
+    with monkeypatch.context() as mp:
+        mp.setattr(pool, "ref_count", None)
+        rows, pos = bm.reserve([0, 1, 2], [1, 5, 1])
+        assert bm.shared_prefix([0, 1, 2]) == ([], 0)
+    assert pos == [14, 14, 15, 16, 17, 18, 14] and bm.seq_len(1) == 19
+    assert bm.shared_prefix([]) == ([], 0)
+    bm._pages = {s: list(c) for s, c in bm._pages.items()}
+    bm.fork_sequence(0, 3)
+    assert bm.shared_prefix([0, 3]) == (bm.sequence_page_chain(0)[:3], 12)
+    bm.reserve([3, 0], [1, 1])  # the last, partly filled page is copied
+    assert bm.sequence_page_chain(0)[:3] == bm.sequence_page_chain(3)[:3]
+    assert bm.sequence_page_chain(0)[3] != bm.sequence_page_chain(3)[3]
