@@ -18,8 +18,9 @@
 //
 // Measured: 256 sequences of 8 drafts over 131072 tokens (246 MB of rows) 61 us, 4.0 TB/s, 0.61 of the device's
 // copy rate: a CTA reads its 131 KB only after the accepted drafts are known and is idle in the two exchanges
-// behind it (an order of steps, which reads of the next sequence's row could fill, not a bound of the device). 64 of 5 over 50257 in bf16 12 us and one of 4 in fp32 8 us: the chain tokens -> gathers -> row ->
-// sums -> segment, five dependent trips to memory.
+// behind it (an order of steps, which reads of the next sequence's row could fill, not a bound of the device).
+// 64 of 5 over 50257 in bf16 12 us and one of 4 in fp32 8 us: the chain tokens -> gathers -> row -> sums ->
+// segment, five dependent trips to memory.
 //
 // Reference parity: scirs2-neural/src/inference/speculative/rejection_sampling.rs:180-330
 // (SpeculativeDecoder::rejection_sampling_step, one sequence on the host).

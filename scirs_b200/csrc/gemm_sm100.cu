@@ -963,7 +963,8 @@ static void launch_tp(int a_mn, int b_mn, int epi, const Maps& m, const PeerMaps
   else if (!a_mn && b_mn && epi == EPI_BF16) launch_tp_t<0, 1, EPI_BF16>(m, pm, args, grid, s);
   else if (!a_mn && b_mn && epi == EPI_DGELU) launch_tp_t<0, 1, EPI_DGELU>(m, pm, args, grid, s);
   else if (a_mn && b_mn && epi == EPI_F32) launch_tp_t<1, 1, EPI_F32>(m, pm, args, grid, s);
-  else TORCH_CHECK(false, "tensor-parallel GEMM form not supported: a_mn=", num(a_mn), " b_mn=", num(b_mn), " epi=", num(epi));
+  else TORCH_CHECK(false, "tensor-parallel GEMM form not supported: a_mn=", num(a_mn), " b_mn=", num(b_mn),
+                   " epi=", num(epi));
 }
 
 // EPI_ROPE arguments: fp32 [S, hd/2] cos / sin tables, hd a multiple of 64

@@ -72,7 +72,8 @@ CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, uint64_t i
                                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", num((int)r), " (inner=", num(inner),
-              " outer=", num(outer), " stride=", num(row_stride_bytes), " box=", num(box_inner), "x", num(box_outer), ")");
+              " outer=", num(outer), " stride=", num(row_stride_bytes), " box=", num(box_inner), "x",
+              num(box_outer), ")");
   return m;
 }
 

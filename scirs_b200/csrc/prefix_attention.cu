@@ -617,9 +617,9 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 
 }  // namespace prefix
 
-// q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape, and the launches made. Pools [num_pages, block_size,
-// Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B], pages int32
-// [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
+// q [B, Q, H, HD] or [B, H, HD] (one query a sequence) bf16 -> the same shape, and the launches made. Pools
+// [num_pages, block_size, Hkv, HD] bf16; tables int32 [B, max_pages] (each sequence's whole chain), lens int32 [B],
+// pages int32 [>= ceil(L / block_size)] (the prefix's chain), qlens int32 [B] or none.
 // tcgen05 takes the prefix from kTcKeys keys on if more than kTcRows rows share a cached head, and from kTcLong
 // keys on always (8 cached heads of 128, tails of 128, mma.sync -> tcgen05: 24 rows, 1024 keys 15.8 -> 14.8 us,
 // 8192 keys 37 -> 25 us; 16 rows, 8192 keys 21 -> 23 us, 65536 keys 66 -> 60 us; 16 rows of heads of 64, 1024 keys
@@ -628,11 +628,11 @@ constexpr int64_t kTcRows = 16, kTcKeys = 512, kTcLong = 32768;
 // Keys of an item, at least (16 rows, 1024 keys of the prefix: 256 instead of 128 takes 12.8 us, not 10.8), and
 // parts of a row's prefix, at most, where they fill the device (8192 keys in 32 parts instead of 64: 22 -> 15 us).
 constexpr int64_t kMinKeys = 128, kParts = 32;
-// Keys that a warp of a sequence that ends inside the prefix walks, at most, before spare items take parts of them (2048
-// take 0.15 ms). With one such sequence of 99990 tokens of 16 a call takes 181 us, without spare items 1484; 3 of 256
-// inside 32768 tokens 311 us, not 705; in tails of a warp 155, not 1616. Where no sequence ends inside, the kernels with
-// spare items cost 0.3 to 1 % behind long prefixes, but 4 to 7 % where items are short or have 32 rows (1024 sequences
-// behind 2048 tokens 94 -> 101 us, 64 x 5 x 8 heads behind 4096 118 -> 123): those go without.
+// Keys that a warp of a sequence that ends inside the prefix walks, at most, before spare items take parts of them
+// (2048 take 0.15 ms). With one such sequence of 99990 tokens of 16 a call takes 181 us, without spare items 1484; 3 of
+// 256 inside 32768 tokens 311 us, not 705; in tails of a warp 155, not 1616. Where no sequence ends inside, the kernels
+// with spare items cost 0.3 to 1 % behind long prefixes, but 4 to 7 % where items are short or have 32 rows (1024
+// sequences behind 2048 tokens 94 -> 101 us, 64 x 5 x 8 heads behind 4096 118 -> 123): those go without.
 constexpr int64_t kWalk = 2048;
 // Up to here a warp joins a row's parts, above four do (2048 rows of 20 parts: 9 us with four).
 constexpr int kFewParts = 8;

@@ -184,8 +184,8 @@ class GPTGenerator:
             bt, sl, pages, shared = self._cache_of(seq_ids)
 
             def attend(q, pool):
-                # Forked sequences: the pages they all begin with are read once. One shared page is enough: 2 to 64
-                # sequences of 40 to 1000 tokens, 12 heads of 64, 16 to 976 shared: 11 to 73 us, by themselves 20 to 214.
+                # Forked sequences: the pages they all begin with are read once. One shared page is enough: 2 to
+                # 64 sequences of 40 to 1000 tokens, 12 heads of 64, 16 to 976 shared 11 to 73 us, else 20 to 214.
                 if shared:
                     return self.attn.forward_shared_prefix(q, pool, bt, sl, pages, shared)
                 return self.attn.forward_batch(q.contiguous(), pool, bt, sl)

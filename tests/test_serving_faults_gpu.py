@@ -186,7 +186,7 @@ def test_a_block_of_bad_prefix_pages():
         assert ((out - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -11) * a).all()
 
 
-# ------------------------------------------------------------------------------------------------ shorter than the prefix
+# ------------------------------------------------------------------------------------------------ inside the prefix
 @pytest.mark.parametrize("lens,Q,Hkv,G,HD,bs,L,qlens", [
     # tcgen05 takes the prefix; one, some, most and all of the sequences end inside it
     pytest.param([2100] * 19 + [2040], 1, 2, 2, 128, 16, 2048, None, id="one_of_twenty"),
@@ -201,7 +201,8 @@ def test_a_block_of_bad_prefix_pages():
     pytest.param([3000, 2980, 2, 2999], 2, 1, 2, 128, 5, 2990, [2, 2, 1, 2], id="items_cp_async"),
     # a warp a tail
     pytest.param([1300 if i % 9 else 1100 + i for i in range(100)], 1, 16, 1, 64, 16, 1250, None, id="warps"),
-    pytest.param([1300 if i % 50 else 900 for i in range(100)], 2, 16, 1, 128, 16, 1250, [1 + i % 2 for i in range(100)], id="warps_two_queries"),
+    pytest.param([1300 if i % 50 else 900 for i in range(100)], 2, 16, 1, 128, 16, 1250, [1 + i % 2 for i in range(100)],
+                 id="warps_two_queries"),
     pytest.param([20000, 20040, 19000], 1, 8, 8, 128, 16, 20010, None, id="long"),
     # more keys than one item takes
     pytest.param([9100] * 11 + [9000], 1, 1, 2, 128, 16, 9040, None, id="long_one_of_twelve"),
@@ -213,7 +214,8 @@ def test_a_block_of_bad_prefix_pages():
     pytest.param([9100, 9000, 8500], 1, 2, 4, 64, 16, 9040, None, id="long_items"),
     pytest.param([9100, 9000, 8500], 2, 1, 2, 128, 5, 9040, [2, 2, 1], id="long_items_cp_async"),
     pytest.param([2300 if i % 9 else 2100 + i for i in range(100)], 1, 16, 1, 64, 16, 2250, None, id="long_warps"),
-    pytest.param([2300 if i % 50 else 2200 for i in range(100)], 2, 16, 1, 128, 16, 2250, [1 + i % 2 for i in range(100)], id="long_warps_two_queries"),
+    pytest.param([2300 if i % 50 else 2200 for i in range(100)], 2, 16, 1, 128, 16, 2250, [1 + i % 2 for i in range(100)],
+                 id="long_warps_two_queries"),
 ])
 def test_sequences_that_end_inside_a_long_prefix(lens, Q, Hkv, G, HD, bs, L, qlens):
     c = Case(lens, Q, Hkv, G, HD, bs, L, qlens, seed=L + Q)
@@ -241,7 +243,7 @@ def test_a_sequence_that_ends_inside_the_prefix_in_a_graph():
 
 
 def test_a_sequence_that_ends_inside_the_prefix_does_not_hold_up_the_batch():
-    """Read by one item it took 14 times what the others take; the parts that the device's items share, less than twice."""
+    """Read by one item it took 14 times what the others take; in parts that spare items share, less than twice."""
     B, Hkv, G, HD, bs, L = 16, 8, 5, 128, 16, 65536
     n = L // bs
     pool = KvPagePool(2 * n + B, KvPageConfig(block_size=bs, num_heads=Hkv, head_dim=HD), DEV)
